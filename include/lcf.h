@@ -681,6 +681,100 @@ int lcf_lc_dp_design(const float *ulookup, int n_lookup, const int *node_k,
                      const double *theta_las, int T, int N, double max_dtheta, int *choice,
                      void *ws, size_t ws_bytes, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Row operators of a training step and of serving (no counterpart in the reference but the clip,
+ * second/pytorch/train.py:342).  Element types of rows: */
+#define LCF_F32 0
+#define LCF_BF16 1
+#define LCF_F16 2
+/* and of rows stored in 8 bits (OCP): */
+#define LCF_E4M3 0
+#define LCF_E5M2 1
+
+/* The norm of many gradient tensors at once, and clipping by it.  `grads` is a HOST array, read
+ * before the call returns: g [n] elements of `dtype` in memory order (a dense tensor of any
+ * shape), out [n] elements of out_dtype (the clipped gradient; out == g with the same type clips
+ * in place; ignored by lcf_grad_norm).  Tensors need no alignment beyond their elements'; n may be
+ * 0.  An output may not overlap a gradient (other than its own, exactly) or another output:
+ * LCF_ERR_ARG.
+ * norm [1] = (sum |g|^p)^(1/p) over all elements, p = 1 or 2, or the largest |g| (p = 0 stands for
+ * infinity), summed in 64 bits over a fixed partition: run-to-run identical, and squares neither
+ * overflow nor vanish.  lcf_grad_clip also writes
+ *   out = g * min(1, max_norm / (norm + 1e-6)),
+ * what torch.nn.utils.clip_grad_norm_ computes (a NaN norm makes every output NaN, an infinite
+ * one makes them 0, or NaN where g is not finite).  ws: lcf_grad_norm_workspace_bytes(count). */
+typedef struct lcf_grad {
+    const void *g;
+    void *out;
+    long long n;
+    int dtype, out_dtype;
+} lcf_grad;
+size_t lcf_grad_norm_workspace_bytes(int count);
+int lcf_grad_norm(const lcf_grad *grads, int count, int p, float *norm, void *ws, size_t ws_bytes,
+                  void *stream);
+int lcf_grad_clip(const lcf_grad *grads, int count, int p, float max_norm, float *norm, void *ws,
+                  size_t ws_bytes, void *stream);
+
+/* Root-mean-square norm of rows with the residual's addition.
+ *   h = round(x + residual)        (h = x when residual is NULL; h is then not written)
+ *   inv = 1 / sqrt(mean(h^2) + eps)
+ *   y = h * inv * weight           (weight NULL = ones)
+ * x, residual [rows, width] of `dtype`, `ldx` / `ldr` elements between rows; y, h contiguous, of
+ * the same type; either may be NULL.  weight [width] of weight_dtype.  inv [rows] fp32 (NULL = not
+ * wanted) is what the backward pass needs.  q8 != NULL: y also (or only) as 8-bit rows of format
+ * `fmt` with one E8M0 scale byte for each 128 columns, from the unrounded fp32 y: row r at
+ * q8 + r * ldq (ldq a multiple of 16 and >= width; the bytes between width and the next multiple
+ * of 16 are written as zeros), its scales at scale + r * lds (lds a multiple of 4, >=
+ * ceil(width / 128)); the scale bytes behind the last block are written as zeros.
+ * bwd: g = dy * weight, dx = inv * (g - h * inv^2 * mean(g * h)) + dh (dh NULL = zeros), the
+ * gradient of x and of residual alike; dweight [width] of weight_dtype = sum over the rows of
+ * dy * h * inv, in a fixed order (NULL = not wanted; ws is then not used).  h, dy, dh have strides
+ * ldh, lddy, lddh between rows; dx is contiguous.
+ * Sums in fp32 (dweight's last stage in 64 bits).  1 <= width <= 16384 (LCF_ERR_UNSUPPORTED).
+ * rows == 0: nothing but dweight = 0. */
+int lcf_rms_norm_fwd(const void *x, long long ldx, const void *residual, long long ldr, int rows,
+                     int width, int dtype, const void *weight, int weight_dtype, float eps, void *y,
+                     void *h, float *inv, void *q8, long long ldq, unsigned char *scale, int lds,
+                     int fmt, void *stream);
+size_t lcf_rms_norm_workspace_bytes(int rows, int width);
+int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long lddy, const void *dh,
+                     long long lddh, int rows, int width, int dtype, const void *weight,
+                     int weight_dtype, const float *inv, void *dx, void *dweight, void *ws,
+                     size_t ws_bytes, void *stream);
+
+/* 8-bit rows with a power-of-two scale for each block of 128, and their product.
+ * A matrix [R, C] in 8-bit form is bytes q (row r at q + r * ld, ld a multiple of 16, the buffer
+ * holding R * ld bytes) and E8M0 scale bytes s (s + r * lds, lds a multiple of 4): element (r, c)
+ * stands for q[r][c] * 2^(s[r][c / 128] - 127), or with 128-row scale blocks
+ * q[r][c] * 2^(s[r / 128][c / 128] - 127).  2^e is the smallest power of two that brings the
+ * block's largest finite magnitude inside the format (448 for e4m3, 57344 for e5m2), e >= -126;
+ * a block of zeros has e = 0; infinities and NaN are stored as NaN and do not enter the scale.
+ * quant: x [R, C] (ldx elements between rows) ->
+ *   rows form (q / s, NULL = not wanted), blocks of 1 x 128 along each row, and / or
+ *   columns form (qt / st, NULL = not wanted): the rows form of x^T, [C, R], blocks of 128 along
+ *   each column; square != 0: one scale for 128 x 128, and s / st have ceil(R / 128) /
+ *   ceil(C / 128) rows.
+ *   Bytes between the last column and the next multiple of 16, and scale bytes between the last
+ *   block and the next multiple of 4, are written as zeros.
+ * gemm: out[m][n] = act((sum_k a[m][k] b[n][k]) * scale[n] + shift[n]), a [M, K], b [N, K] in rows
+ *   form, b_square != 0: b has 128 x 128 scale blocks; scale / shift fp32 or NULL, relu != 0 clamps
+ *   at 0; out [M, N] of out_dtype, ldo elements between rows.  What lies in a row behind column K
+ *   does not enter.  out_dtype fp32: exact products summed in fp32 (bytes widened to bf16 in
+ *   registers); bf16 / fp16: the 8-bit matrix instructions, whose sums of eight neighbouring
+ *   products keep 13 bits below the largest of them (an error of at most 2^-10 of the sum of
+ *   magnitudes; about 1.5e-5 of the result on random data), then one rounding.
+ *   K == 0 gives act(shift).  ws: lcf_f8_gemm_workspace_bytes(M, N, K) (0 for most sizes: the sum
+ *   is split over workgroups only where the output has few tiles; the parts are joined in a fixed
+ *   order, so results are run-to-run identical). */
+int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtype, int fmt, int square, void *q,
+                 long long ldq, unsigned char *s, int lds, void *qt, long long ldqt,
+                 unsigned char *st, int ldst, void *stream);
+size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K);
+int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa, int ldsa, int a_fmt,
+                const void *b, long long ldb, const unsigned char *sb, int ldsb, int b_fmt,
+                int b_square, int M, int N, int K, const float *scale, const float *shift, int relu,
+                void *out, long long ldo, int out_dtype, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@ if os.environ.get("LCF_LIB"):  # an experimental build of the same library (A/B 
 c_int = ctypes.c_int
 c_size_t = ctypes.c_size_t
 c_void_p = ctypes.c_void_p
+c_ll = ctypes.c_longlong
 _I3 = ctypes.c_int * 3
 _F3 = ctypes.c_float * 3
 _F6 = ctypes.c_float * 6
@@ -189,6 +190,23 @@ SYMBOLS = {
     "lcf_bn_relu_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p,
                                 c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                 c_void_p]),
+    "lcf_grad_norm_workspace_bytes": (c_size_t, [c_int]),
+    "lcf_grad_norm": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "lcf_grad_clip": (c_int, [c_void_p, c_int, c_int, ctypes.c_float, c_void_p, c_void_p, c_size_t,
+                              c_void_p]),
+    "lcf_rms_norm_fwd": (c_int, [c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_int, c_void_p,
+                                 c_int, ctypes.c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_ll, c_void_p, c_int, c_int, c_void_p]),
+    "lcf_rms_norm_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "lcf_rms_norm_bwd": (c_int, [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_int, c_int,
+                                 c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_size_t, c_void_p]),
+    "lcf_f8_quant": (c_int, [c_void_p, c_ll, c_int, c_int, c_int, c_int, c_int, c_void_p, c_ll,
+                             c_void_p, c_int, c_void_p, c_ll, c_void_p, c_int, c_void_p]),
+    "lcf_f8_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "lcf_f8_gemm": (c_int, [c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_ll, c_void_p,
+                            c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
+                            c_void_p, c_ll, c_int, c_void_p, c_size_t, c_void_p]),
 }
 
 # entry points whose LAST argument is the caller's lcf_ctx (NULL = defaults): the binding lets

@@ -1,0 +1,128 @@
+"""CPU: what the row operators refuse, before anything reaches a GPU, and the 64-bit forms that the
+GPU tests compare with against known answers."""
+import ctypes
+
+import pytest
+import torch
+
+import row_reference as ref
+from objectdetection_amd import _lib, ops
+
+ARG, WORKSPACE, UNSUPPORTED = -1, -2, -3
+
+
+def test_reference_8_bit_form_on_known_values():
+    v = torch.zeros((2, 130))
+    v[0, 0], v[0, 1], v[0, 2] = 448.0, 17.0, 19.0   # 17 lies between 16 and 18, 19 between 18 and 20: to even
+    v[0, 128] = 2.0
+    v[1, 5] = 450.0
+    q, e = ref.quantise(v)
+    assert e.tolist() == [[0, -7], [1, 0]]  # 2 = 256 * 2^-7; a block of zeros has e = 0
+    assert q[0, :3].tolist() == [448.0, 16.0, 20.0] and q[0, 128] == 256.0
+    assert q[1, 5] == 224.0  # 225 lies between 224 and 240
+    for dt in ref.MAX8:  # the same values through torch's own conversion
+        x = torch.randn((5, 256), generator=torch.Generator().manual_seed(1)) * 3
+        q, e = ref.quantise(x, dt)
+        s = (2.0 ** e.float()).repeat_interleave(128, 1)
+        assert torch.equal(q, (x / s).to(dt).double())
+        assert float(q.abs().max()) <= ref.MAX8[dt]
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros((4, 8)), torch.zeros((8,))
+    w8 = (torch.zeros((3, 8)).to(torch.float8_e4m3fn), torch.zeros((3, 1), dtype=torch.uint8))
+    for call in (lambda: ops.rms_norm(x, w), lambda: ops.rms_norm_f8(x, w), lambda: ops.f8_rows(x),
+                 lambda: ops.f8_weight_image(x), lambda: ops.f8_linear(x, torch.zeros((3, 8))),
+                 lambda: ops.f8_matmul(w8, w8), lambda: ops.grad_norm([x]), lambda: ops.clip_norm_([x], 1.0)):
+        with pytest.raises(RuntimeError):
+            call()
+    assert ops.grad_norm([]).item() == 0.0 and ops.clip_norm_([], 1.0).item() == 0.0
+    with pytest.raises(ValueError):
+        ops.grad_norm([x], 3.0)
+    with pytest.raises(ValueError):
+        ops.clip_norm_([x], -1.0)
+
+
+def _grads(*entries):
+    class G(ctypes.Structure):
+        _fields_ = [("g", ctypes.c_void_p), ("out", ctypes.c_void_p), ("n", ctypes.c_longlong),
+                    ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int)]
+    return (G * len(entries))(*[G(*e) for e in entries])
+
+
+def test_abi_refuses_bad_gradient_tables():
+    L = _lib.lib()
+    norm, ws = 4096, 8192  # never touched: every call below is refused on the host
+    room = L.lcf_grad_norm_workspace_bytes(2)
+
+    def clip(*entries, p=2, m=1.0, bytes=room, count=None):
+        t = _grads(*entries)
+        return L.lcf_grad_clip(ctypes.addressof(t), len(entries) if count is None else count, p, m, norm, ws, bytes,
+                               None)
+    good = (1 << 20, 1 << 21, 100, 0, 0)
+    assert clip(good, p=3) == ARG and clip(good, m=-1.0) == ARG and clip(good, m=float("nan")) == ARG
+    assert clip(good, count=-1) == ARG
+    assert clip((0, 1 << 21, 100, 0, 0)) == ARG and clip((1 << 20, 0, 100, 0, 0)) == ARG
+    assert clip((1 << 20, 1 << 21, -1, 0, 0)) == ARG and clip((1 << 20, 1 << 21, 100, 3, 0)) == ARG
+    assert clip((1 << 20, 1 << 21, 100, 0, 7)) == ARG
+    assert clip(good, bytes=16) == WORKSPACE
+    # outputs that overlap another output, a gradient, or their own gradient but not exactly
+    assert clip(good, (1 << 22, (1 << 21) + 396, 100, 0, 0)) == ARG
+    assert clip(good, ((1 << 21) + 396, 1 << 23, 100, 0, 0)) == ARG
+    assert clip((1 << 20, (1 << 20) + 4, 100, 0, 0)) == ARG
+    assert clip((1 << 20, 1 << 20, 100, 0, 1)) == ARG
+    assert clip((1 << 20, 1 << 20, 100, 0, 0), (1 << 20, 1 << 20, 100, 0, 0)) == ARG
+    t = _grads(good)
+    assert L.lcf_grad_norm(ctypes.addressof(t), 1, 2, None, ws, room, None) == ARG
+    assert L.lcf_grad_norm(ctypes.addressof(t), 1, 2, norm, ws, 8, None) == WORKSPACE
+
+
+def test_abi_refuses_bad_norm_arguments():
+    L = _lib.lib()
+
+    def fwd(x=4096, ldx=64, r=None, ldr=0, rows=4, width=64, dt=0, w=None, wd=0, eps=1e-6, h=None, q8=None, ldq=64,
+            s=None, lds=4, fmt=0):
+        return L.lcf_rms_norm_fwd(x, ldx, r, ldr, rows, width, dt, w, wd, eps, 8192, h, None, q8, ldq, s, lds, fmt,
+                                  None)
+    for bad in (dict(x=None), dict(ldx=63), dict(rows=-1), dict(width=0), dict(dt=3), dict(w=4096, wd=9),
+                dict(r=4096, ldr=10), dict(h=4096), dict(eps=-1.0), dict(eps=float("nan")), dict(q8=4096),
+                dict(q8=4096, s=4096, ldq=40), dict(q8=4100, s=4096), dict(q8=4096, s=4096, lds=3),
+                dict(q8=4096, s=4097), dict(q8=4096, s=4096, fmt=2), dict(q8=4096, s=4096, lds=0)):
+        assert fwd(**bad) == ARG, bad
+    assert fwd(width=16385, ldx=16385) == UNSUPPORTED
+    assert fwd(rows=0, x=None) == 0
+
+    def bwd(h=4096, ldh=64, dy=4096, lddy=64, dh=None, lddh=0, rows=4, width=64, dt=0, w=None, wd=0, inv=4096, dx=8192,
+            dw=None, ws=None, n=0):
+        return L.lcf_rms_norm_bwd(h, ldh, dy, lddy, dh, lddh, rows, width, dt, w, wd, inv, dx, dw, ws, n, None)
+    for bad in (dict(h=None), dict(dy=None), dict(inv=None), dict(dx=None), dict(ldh=8), dict(lddy=8),
+                dict(dh=4096, lddh=3), dict(rows=-1), dict(width=0), dict(dt=5), dict(dw=4096, wd=4),
+                dict(dw=4096)):
+        assert bwd(**bad) == ARG, bad
+    assert bwd(dw=4096, ws=4096, n=64) == WORKSPACE
+    assert bwd(width=20000, ldh=20000, lddy=20000) == UNSUPPORTED
+
+
+def test_abi_refuses_bad_8_bit_operands():
+    L = _lib.lib()
+
+    def quant(x=4096, ldx=64, R=4, C=64, dt=0, fmt=0, sq=0, q=4096, ldq=64, s=4096, lds=4, qt=None, ldqt=0, st=None,
+              ldst=0):
+        return L.lcf_f8_quant(x, ldx, R, C, dt, fmt, sq, q, ldq, s, lds, qt, ldqt, st, ldst, None)
+    for bad in (dict(x=None), dict(ldx=10), dict(R=-1), dict(C=-1), dict(dt=7), dict(fmt=2), dict(q=None),
+                dict(q=4104), dict(ldq=56), dict(ldq=48), dict(s=None), dict(s=4098), dict(lds=2),
+                dict(qt=4096), dict(qt=4096, ldqt=16, st=4096, ldst=3), dict(qt=4096, ldqt=8, st=4096, ldst=4)):
+        assert quant(**bad) == ARG, bad
+    assert quant(R=0, x=None) == 0 and quant(C=0, x=None) == 0
+    assert quant(R=1 << 30, sq=1) == UNSUPPORTED
+
+    def gemm(a=4096, lda=64, sa=4096, ldsa=4, af=0, b=4096, ldb=64, sb=4096, ldsb=4, bf=0, sq=0, M=4, N=4, K=64,
+             out=8192, ldo=4, od=0, ws=None, n=0):
+        return L.lcf_f8_gemm(a, lda, sa, ldsa, af, b, ldb, sb, ldsb, bf, sq, M, N, K, None, None, 0, out, ldo, od, ws,
+                             n, None)
+    for bad in (dict(a=None), dict(lda=60), dict(lda=48), dict(a=4097), dict(sa=None), dict(ldsa=1), dict(af=2),
+                dict(b=None), dict(ldb=63), dict(sb=4097), dict(bf=5), dict(M=-1), dict(K=-1), dict(out=None),
+                dict(ldo=3), dict(od=3), dict(K=70000, lda=70016, ldb=70016, ldsa=548, ldsb=548)):
+        assert gemm(**bad) == ARG, bad
+    assert gemm(K=70000, lda=70016, ldb=70016, ldsa=548, ldsb=548, ws=4096, n=16) == WORKSPACE
+    assert gemm(M=0, a=None) == 0 and gemm(N=0, b=None) == 0
