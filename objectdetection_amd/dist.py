@@ -112,8 +112,28 @@ class FlatGradAllReduce:
     def clip_norm_(self, max_norm):
         """torch.nn.utils.clip_grad_norm_ over all parameters, on the flat buffer: the 2-norm of
         the concatenation is the norm of the per-tensor norms.  Returns the total norm."""
+        if self.flat.is_cuda:
+            from . import ops
+            return ops.clip_norm_([self.flat], max_norm)
         total = torch.linalg.vector_norm(self.flat)
         self.flat.mul_(torch.clamp(max_norm / (total + 1e-6), max=1.0))
+        return total
+
+    def collect_clip_(self, max_norm):
+        """collect() and clip_norm_() of a step without an exchange between them (one rank): the
+        norm is taken over the gradients as autograd produced them and the clipped values are what
+        is copied into the buffer -- one reading and one writing of the buffer less."""
+        params = self.params
+        views = [v for vs in self.views for v in vs]
+        if self.attach or not self.flat.is_cuda or any(
+                p.grad is None or p.grad is v or p.grad.stride() != v.stride()
+                for p, v in zip(params, views)):
+            self.collect()
+            return self.clip_norm_(max_norm)
+        from . import ops
+        total = ops.clip_norm_([p.grad for p in params], max_norm, out=self.flat)
+        for p, v in zip(params, views):
+            p.grad = v
         return total
 
     def reduce(self, segment=None, async_op=False):

@@ -400,11 +400,14 @@ class conv_math:
     accumulate, tolerance 2e-2); "bf16x3" for INFERENCE (the no-grad forward of the sparse conv
     modules with split hi + lo bf16 operands, fp32 tolerance; "bf16x8": three exact planes and
     eight products, fp32-grade; training under either stays fp32).
-    Layers whose channels are not 32/64/128 stay fp32 in every mode."""
+    Layers whose channels are not 32/64/128 stay fp32 in these modes.  "f8": POINTWISE convs (an
+    all-ones kernel at stride 1, any channel counts) in 8-bit form with a scale for each block of
+    128, training and inference (``f8_linear`` / ``f8_matmul``; tolerance: half a step of e4m3 for
+    each operand); every other layer as in "f32"."""
 
     def __init__(self, mode):
-        if mode not in ("f32", "bf16", "bf16x3", "bf16x8"):
-            raise ValueError("conv math mode must be 'f32', 'bf16', 'bf16x3' or 'bf16x8'")
+        if mode not in ("f32", "bf16", "bf16x3", "bf16x8", "f8"):
+            raise ValueError("conv math mode must be 'f32', 'bf16', 'bf16x3', 'bf16x8' or 'f8'")
         self.mode, self.prev = mode, None
 
     def __enter__(self):
@@ -1283,7 +1286,7 @@ def _norm_args(tensors, norm_type):
     if not tensors:
         return tensors, None, None, None
     where = {t.get_device() for t in tensors}
-    if where == {-1} or -1 in where:
+    if -1 in where:
         _need_cuda(*tensors)
     if len(where) != 1:
         raise RuntimeError("the tensors of one norm must be on one device")
@@ -1656,15 +1659,17 @@ def f8_matmul(a, b, scale=None, shift=None, relu=False, out_dtype=torch.float32,
 class F8LinearFunction(torch.autograd.Function):
     """y = x W^T (+ bias) with x and W rounded to 8-bit form; the three products (y, dx = dy W,
     dW = dy^T x) run on 8-bit operands with fp32 accumulation, each operand's scale blocks lying
-    along the axis that its product sums over.  The rounding is passed through unchanged."""
+    along the axis that its product sums over.  The rounding is passed through unchanged.
+    ``turned``: the weight is stored [K, N], as sparse convs store it."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        y = f8_matmul(f8_rows(x), f8_weight_image(weight),
+    def forward(ctx, x, weight, bias, turned, x8):
+        y = f8_matmul(f8_rows(x) if x8 is None else x8, f8_weight_image(weight, transpose=turned),
                       shift=None if bias is None else bias.detach().float().contiguous(),
                       out_dtype=x.dtype)
         ctx.save_for_backward(x, weight)
         ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.turned = turned
         return y
 
     @staticmethod
@@ -1676,26 +1681,32 @@ class F8LinearFunction(torch.autograd.Function):
         rows, cols = _f8_quant(dy, torch.float8_e4m3fn, False, need_x, need_w) \
             if need_x or need_w else (None, None)
         if need_x:
-            dx = f8_matmul(rows, f8_weight_image(weight, transpose=True), out_dtype=x.dtype)
+            dx = f8_matmul(rows, f8_weight_image(weight, transpose=not ctx.turned),
+                           out_dtype=x.dtype)
         if need_w:
-            dw = f8_matmul(cols, f8_cols(x), out_dtype=weight.dtype)
+            pair = (f8_cols(x), cols) if ctx.turned else (cols, f8_cols(x))
+            dw = f8_matmul(*pair, out_dtype=weight.dtype)
         if ctx.bias_dtype is not None and ctx.needs_input_grad[2]:
             db = dy.float().sum(0).to(ctx.bias_dtype)
-        return dx, dw, db
+        return dx, dw, db, None, None
 
 
-def f8_linear(x, weight, bias=None):
+def f8_linear(x, weight, bias=None, turned=False, x8=None):
     """x [..., K] (float32, bfloat16 or float16) times weight [N, K]^T (+ bias [N]) on 8-bit
     operands: -> [..., N] of x's type, differentiable in all three (weight and bias keep their own
-    types).  Error of an operand: half a step of e4m3, 2^-4 of a value, plus 2^-10 of its block's
-    scale for small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
+    types).  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.
+    Error of an operand: half a step of e4m3, 2^-4 of a value, plus 2^-10 of its block's scale for
+    small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
     _need_cuda(x, weight, bias)
     if x.dtype not in _TYPE_CODE or weight.dtype not in _TYPE_CODE or weight.dim() != 2 or \
-            x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+            x.dim() < 1 or x.shape[-1] != weight.shape[0 if turned else 1]:
         raise ValueError(f"f8_linear: x {tuple(x.shape)} {x.dtype} against weight "
                          f"{tuple(weight.shape)} {weight.dtype}")
-    if bias is not None and (tuple(bias.shape) != (weight.shape[0],)
-                             or not bias.dtype.is_floating_point):
-        raise ValueError(f"f8_linear: bias must have {weight.shape[0]} elements")
-    y = F8LinearFunction.apply(x.reshape(-1, x.shape[-1]), weight, bias)
-    return y.view(*x.shape[:-1], weight.shape[0])
+    n = weight.shape[1 if turned else 0]
+    if bias is not None and (tuple(bias.shape) != (n,) or not bias.dtype.is_floating_point):
+        raise ValueError(f"f8_linear: bias must have {n} elements")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x8 is not None and tuple(x8[0].shape) != tuple(x2.shape):
+        raise ValueError("f8_linear: x8 must be the 8-bit form of x")
+    y = F8LinearFunction.apply(x2, weight, bias, bool(turned), x8)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)

@@ -8,7 +8,8 @@ Make it importable under the name ``spconv`` with ``objectdetection_amd.dropin.i
 from . import ops, utils  # noqa: F401
 from .conv import (SparseConv2d, SparseConv3d, SparseConvolution, SubMConv2d,  # noqa: F401
                    SubMConv3d)
-from .modules import SparseModule, SparseSequential, ToDense, is_spconv_module  # noqa: F401
+from .modules import (RMSNorm, SparseModule, SparseSequential, ToDense,  # noqa: F401
+                      is_spconv_module)
 from .tensor import SparseConvTensor  # noqa: F401
 
 __version__ = "1.1+lcf"

@@ -97,25 +97,29 @@ class SparseConvolution(SparseModule):
                 input.indice_dict[self.indice_key] = rb
         return rb
 
-    def forward(self, input, _scale=None, _shift=None, _relu=False):
+    def forward(self, input, _scale=None, _shift=None, _relu=False, _f8=None):
         assert isinstance(input, SparseConvTensor)
         features = input.features
         if not features.is_cuda:
             raise RuntimeError("spconv (objectdetection_amd) runs on the GPU only: no CPU path")
-        if self.conv1x1 and all(st == 1 for st in self.stride):
+        if self.pointwise:
             # spconv 1.x's short cut for an all-ones kernel (SparseConvolution.forward; used by
             # second/pytorch/models/resnet.py:20-29,69-110): a plain row-wise GEMM, no rulebook --
-            # a library GEMM, so any channel count (SparseBottleneck's 256) goes through
+            # a library GEMM, so any channel count (SparseBottleneck's 256) goes through; under
+            # ops.conv_math("f8") the product on 8-bit rows with its fused epilogue
             w = self.weight.view(self.in_channels, self.out_channels)
-            out = torch.mm(features, w.to(features.dtype))
-            if self.bias is not None:
-                out = out + self.bias.to(out.dtype)
-            if _scale is not None:
-                out = out * _scale.to(out.dtype)
-            if _shift is not None:
-                out = out + _shift.to(out.dtype)
-            if _relu:
-                out = torch.relu(out)
+            if ops.get_conv_math() == "f8":
+                out = self._pointwise_f8(features, w, _scale, _shift, _relu, _f8)
+            else:
+                out = torch.mm(features, w.to(features.dtype))
+                if self.bias is not None:
+                    out = out + self.bias.to(out.dtype)
+                if _scale is not None:
+                    out = out * _scale.to(out.dtype)
+                if _shift is not None:
+                    out = out + _shift.to(out.dtype)
+                if _relu:
+                    out = torch.relu(out)
             out_tensor = SparseConvTensor(out, input.indices, input.spatial_shape,
                                           input.batch_size)
             out_tensor.indice_dict = input.indice_dict
@@ -153,6 +157,26 @@ class SparseConvolution(SparseModule):
         out_tensor.grid = input.grid
         return out_tensor
 
+    @property
+    def pointwise(self):
+        """A row-wise linear layer: no rulebook, no neighbours."""
+        return self.conv1x1 and all(st == 1 for st in self.stride)
+
+    def _pointwise_f8(self, x, w, scale, shift, relu, f8):
+        """Rows x [K, Cin] (or, in inference, their 8-bit form ``f8`` already) through w [Cin, Cout]
+        on 8-bit operands."""
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad):
+            out = ops.f8_linear(x, w, self.bias, turned=True)
+            return torch.relu(out) if relu else out
+        if self.bias is not None:
+            b = self.bias.detach().float()
+            b = b if scale is None else b * scale
+            shift = b if shift is None else b + shift
+        return ops.f8_matmul(
+            ops.f8_rows(x) if f8 is None else f8, self._weight_image("f8"),
+            None if scale is None else scale.float().contiguous(),
+            None if shift is None else shift.float().contiguous(), relu, out_dtype=x.dtype)
+
     def _inference_forward(self, x, rb, scale, shift, relu):
         """No-grad forward: fp32 MFMA, or -- under ``ops.conv_math("bf16x3")`` and for 32 / 64 /
         128 channels on both sides -- split bf16 operands at fp32 tolerance (include/lcf.h)."""
@@ -166,14 +190,18 @@ class SparseConvolution(SparseModule):
                                 scale, shift, relu)
 
     def _weight_image(self, planes=0):
-        """MFMA weight image (planes 2 / 3: the split bf16x3 / bf16x8 image), cached until the
-        parameter is modified in place or replaced."""
+        """MFMA weight image (planes 2 / 3: the split bf16x3 / bf16x8 image; "f8": a pointwise conv's
+        8-bit form), cached until the parameter is modified in place or replaced."""
         w = self.weight
         tag = (w.data_ptr(), w._version, w.device, w.dtype)
         name = f"_wimg{planes}"
         cache = getattr(self, name, None)
         if cache is None or cache[0] != tag:
-            img = ops.weight_image_bf16x3(w, planes=planes) if planes else ops.weight_image(w)
+            if planes == "f8":
+                img = ops.f8_weight_image(w.view(self.in_channels, self.out_channels),
+                                          transpose=True)
+            else:
+                img = ops.weight_image_bf16x3(w, planes=planes) if planes else ops.weight_image(w)
             cache = (tag, img)
             object.__setattr__(self, name, cache)
         return cache[1]

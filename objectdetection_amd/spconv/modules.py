@@ -33,6 +33,24 @@ def _bn_affine(bn):
     return scale, shift
 
 
+class RMSNorm(nn.RMSNorm):
+    """Root-mean-square norm of a sparse tensor's rows [K, C] (an ordinary nn.Module: inside a
+    SparseSequential it runs on ``.features``), optionally with the residual's addition of a
+    SparseBasicBlock (second/pytorch/models/resnet.py:54-64): ``norm(x, residual)`` ->
+    (normed, x + residual).  Statistics are per row, so unlike BatchNorm1d it does the same in
+    training and inference and for any number of rows.  eps None: the rows' type's epsilon, as in
+    nn.RMSNorm."""
+
+    def __init__(self, num_features, eps=None, elementwise_affine=True):
+        super().__init__(num_features, eps, elementwise_affine)
+
+    def _eps(self, x):
+        return torch.finfo(x.dtype).eps if self.eps is None else self.eps
+
+    def forward(self, x, residual=None):
+        return ops.rms_norm(x, self.weight, self._eps(x), residual)
+
+
 class SparseSequential(SparseModule):
     """Sequential container that runs sparse modules on the SparseConvTensor and ordinary
     nn.Modules (BatchNorm1d, ReLU, ...) on its ``.features``.
@@ -43,7 +61,8 @@ class SparseSequential(SparseModule):
     Set ``fuse_inference = False`` to run module by module.  In training a
     ``BatchNorm1d (training) -> ReLU`` pair on the features runs as the fused streaming kernels of
     ``ops.bn_relu_train`` (same values and running statistics as the two torch modules;
-    ``fuse_training = False`` to turn it off).
+    ``fuse_training = False`` to turn it off).  Under ``ops.conv_math("f8")`` without gradients an
+    ``RMSNorm -> pointwise sparse conv`` pair hands over 8-bit rows: the norm writes them itself.
     """
     fuse_inference = True
     fuse_training = True
@@ -149,6 +168,16 @@ class SparseSequential(SparseModule):
                     input = module(input, _scale=scale, _shift=shift, _relu=relu)
                     i += n
                     continue
+            if (fuse and isinstance(module, RMSNorm) and isinstance(input, SparseConvTensor)
+                    and ops.get_conv_math() == "f8" and i + 1 < len(mods)
+                    and is_sparse_conv(mods[i + 1]) and mods[i + 1].pointwise):
+                x = input.features
+                f8, _ = ops.rms_norm_f8(x, module.weight, module._eps(x))
+                n, bn, relu = self._fusable(mods, i + 1)
+                scale, shift = _bn_affine(bn) if bn is not None else (None, None)
+                input = mods[i + 1](input, _scale=scale, _shift=shift, _relu=relu, _f8=f8)
+                i += 1 + n
+                continue
             if is_spconv_module(module):
                 input = module(input)
             elif isinstance(input, SparseConvTensor):

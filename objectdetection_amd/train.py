@@ -130,9 +130,13 @@ class TrainStep:
             self.bucket.collect(0)
             self.bucket.reduce(0)
             self.bucket.wait()
-        else:
+        elif self._world() > 1:
             self.bucket.collect()
             self.bucket.reduce()
-        self.bucket.clip_norm_(10.0)  # clip_grad_norm_(parameters, 10.0), train.py:342
+        # clip_grad_norm_(parameters, 10.0), train.py:342
+        if self._world() > 1:
+            self.bucket.clip_norm_(10.0)
+        else:
+            self.bucket.collect_clip_(10.0)
         self.opt.step()
         return loss.detach()
