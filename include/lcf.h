@@ -763,17 +763,25 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  *   registers); bf16 / fp16: the 8-bit matrix instructions, whose sums of eight neighbouring
  *   products keep 13 bits below the largest of them (an error of at most 2^-10 of the sum of
  *   magnitudes; about 1.5e-5 of the result on random data), then one rounding.
- *   K == 0 gives act(shift).  ws: lcf_f8_gemm_workspace_bytes(M, N, K) (0 for most sizes: the sum
+ *   K == 0 gives act(shift).  lda, ldb <= 2^22 (LCF_ERR_UNSUPPORTED).  ws: lcf_f8_gemm_workspace_bytes(M, N, K, out_dtype) (0 for most sizes: the sum
  *   is split over workgroups only where the output has few tiles; the parts are joined in a fixed
  *   order, so results are run-to-run identical). */
 int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtype, int fmt, int square, void *q,
                  long long ldq, unsigned char *s, int lds, void *qt, long long ldqt,
                  unsigned char *st, int ldst, void *stream);
-size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K);
+size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype);
 int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa, int ldsa, int a_fmt,
                 const void *b, long long ldb, const unsigned char *sb, int ldsb, int b_fmt,
                 int b_square, int M, int N, int K, const float *scale, const float *shift, int relu,
                 void *out, long long ldo, int out_dtype, void *ws, size_t ws_bytes, void *stream);
+/* lcf_f8_quant of x (rows form, e4m3) and lcf_f8_gemm against an e4m3 b in ONE launch, the 8-bit rows
+ * staying in registers: the same result bit for bit.  For thin layers over many rows with
+ * dtype == out_dtype: M >= 4096, N <= 256, K <= 512 (fp32: 256) and a multiple of 8, x and its rows
+ * on 4-byte borders; LCF_ERR_UNSUPPORTED otherwise and the caller makes the two calls. */
+int lcf_f8_linear(const void *x, long long ldx, int dtype, const void *b, long long ldb,
+                  const unsigned char *sb, int ldsb, int b_square, int M, int N, int K,
+                  const float *scale, const float *shift, int relu, void *out, long long ldo,
+                  int out_dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -203,7 +203,10 @@ SYMBOLS = {
                                  c_size_t, c_void_p]),
     "lcf_f8_quant": (c_int, [c_void_p, c_ll, c_int, c_int, c_int, c_int, c_int, c_void_p, c_ll,
                              c_void_p, c_int, c_void_p, c_ll, c_void_p, c_int, c_void_p]),
-    "lcf_f8_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "lcf_f8_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "lcf_f8_linear": (c_int, [c_void_p, c_ll, c_int, c_void_p, c_ll, c_void_p, c_int, c_int, c_int,
+                              c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_ll, c_int,
+                              c_void_p]),
     "lcf_f8_gemm": (c_int, [c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_ll, c_void_p,
                             c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
                             c_void_p, c_ll, c_int, c_void_p, c_size_t, c_void_p]),

@@ -49,9 +49,7 @@ template <typename T, int LPB> __global__ void __launch_bounds__(256) f8_rows_ke
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.f;
         if (live && col < p.C) lcf_ld8_tail((const T *)p.x + row * p.ldx, col, p.C, v);
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, lcf_finite_abs(v[i]));
+        float top = lcf_f8_top<8>(v);
 #pragma unroll
         for (int d = LPB / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
         const int e = lcf_f8_exponent(top, p.fmt);
@@ -92,11 +90,12 @@ template <typename T> __global__ void __launch_bounds__(256) f8_tile_kernel(F8Qu
         if (row < p.R && col < p.C) lcf_ld8_tail((const T *)p.x + row * p.ldx, col, p.C, v[i]);
     }
     float cm[8];
+    lcf_f8_top<64>(&v[0][0]); // infinities out first
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         cm[j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cm[j] = fmaxf(cm[j], lcf_finite_abs(v[i][j]));
+        for (int i = 0; i < 8; ++i) cm[j] = fmaxf(cm[j], __builtin_fabsf(v[i][j]));
         cm[j] = fmaxf(cm[j], __shfl_xor(cm[j], 16, 64));
         cm[j] = fmaxf(cm[j], __shfl_xor(cm[j], 32, 64));
     }
@@ -126,7 +125,7 @@ template <typename T> __global__ void __launch_bounds__(256) f8_tile_kernel(F8Qu
             if (!p.square) {
                 float top = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, lcf_finite_abs(v[i][j]));
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, __builtin_fabsf(v[i][j]));
 #pragma unroll
                 for (int d = 8; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
                 e = lcf_f8_exponent(top, p.fmt);
@@ -234,34 +233,41 @@ struct F8Gemm {
     long long lda, ldb, ldo;
     int ldsa, ldsb, b_shift; // b_shift: 7 = one scale row for 128 rows of b
     int M, N, K, relu, code;
-    int tiles_m, tiles_n, ksteps; // ksteps: 128-column steps of one split
+    int tiles_m, tiles_n, splits, ksteps; // ksteps: 128-column steps of one split
 };
 
-__device__ __forceinline__ void f8_store(const F8Gemm &p, long long m, int n, const float *v, int count)
+// `count` (at most W) outputs of row m from column n on: W consecutive columns held by one lane
+template <int W> __device__ __forceinline__ void f8_store(const F8Gemm &p, long long m, int n, const float *v, int count)
 {
-    // v: out columns n .. n + 15 of row m
-    float s[16];
+    float s[W];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float x = v[i];
-        if (i < count) {
-            if (p.scale) x *= p.scale[n + i];
-            if (p.shift) x += p.shift[n + i];
-        }
-        s[i] = p.relu ? (x < 0.f ? 0.f : x) : x; // NaN stays
+    for (int i = 0; i < W; ++i) s[i] = v[i];
+    if (p.scale) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (i < count) s[i] *= p.scale[n + i];
+    }
+    if (p.shift) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (i < count) s[i] += p.shift[n + i];
+    }
+    if (p.relu) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) s[i] = s[i] < 0.f ? 0.f : s[i]; // NaN stays
     }
     auto put = [&](auto *row) {
-        if (count >= 16) {
-            lcf_st8(row, s);
-            lcf_st8(row + 8, s + 8);
+        using T = typename std::remove_pointer<decltype(row)>::type;
+        if (count >= W) {
+            if constexpr (W == 8) lcf_st8(row, s);
+            else *reinterpret_cast<lcf_f4u *>(row) = (lcf_f4u){s[0], s[1], s[2], s[3]};
         } else {
-            using T = typename std::remove_pointer<decltype(row)>::type;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < W; ++i)
                 if (i < count) row[i] = lcf_from_f32<T>(s[i]);
         }
     };
-    if (p.code == LCF_F32) put((float *)p.out + m * p.ldo + n);
+    if constexpr (W == 4) put((float *)p.out + m * p.ldo + n);
     else if (p.code == LCF_BF16) put((lcf_b *)p.out + m * p.ldo + n);
     else put((lcf_h *)p.out + m * p.ldo + n);
 }
@@ -274,6 +280,68 @@ __device__ __forceinline__ void f8_cut(int *w, int col, int K)
         const int left = K - (col + 4 * i);
         if (left <= 0) w[i] = 0;
         else if (left < 4) w[i] &= (1 << (8 * left)) - 1;
+    }
+}
+
+// 16 bytes a lane from a buffer straight to LDS, lane after lane behind `to` (the host's pass does not
+// know the builtin at this width)
+__device__ __forceinline__ void f8_lds16(__amdgpu_buffer_rsrc_t from, unsigned char *to, int off)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, off, 0, 0, 0);
+#endif
+}
+
+// Keeps the four sums of a piece where they are computed.  A matrix instruction reads its operands
+// from all 64 lanes whatever the execution mask says; the compiler moves one that only a guarded
+// store uses into the guarded block, and with it the vector instructions that make its operands,
+// which then run in the storing lanes alone (seen: outputs of a tile that N ends in were wrong).
+// The waits cover the instruction's own latency (at most 19 states before its result may be read).
+__device__ __forceinline__ void f8_pin(f8_f4 (&a)[4])
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
+#endif
+}
+
+template <bool V> struct F8Bool { static constexpr bool value = V; };
+
+// Which of a wave's 64 columns n the row i of its piece t of b stands for.  The instruction's first
+// operand is b, its second a, so lane (r16, g) holds rows i = 4 g + r (r = 0..3) of every piece for
+// one row m of a.  fp32 outputs: n = 16 t + i, four columns (16 bytes) in a piece's four registers.
+// 16-bit outputs: n = 32 (t / 2) + 8 g + 4 (t % 2) + r, eight columns (16 bytes) over two pieces.
+// Either way the four lanes of a row store 64 consecutive bytes at once.
+template <bool WIDE> __device__ __forceinline__ int f8_column(int t, int i)
+{
+    return WIDE ? 16 * t + i : 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
+}
+
+// a wave's 64 columns of row m, from column n0 on, out of its four pieces' sums
+template <bool WIDE> __device__ __forceinline__ void f8_put(const F8Gemm &p, float *ws, long long m, int n0, int g,
+                                                            const f8_f4 *acc)
+{
+    constexpr int W = WIDE ? 4 : 8;
+#pragma unroll
+    for (int q = 0; q < 16 / W; ++q) {
+        const int n = n0 + (WIDE ? 16 * q + 4 * g : 32 * q + 8 * g);
+        float v[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = acc[WIDE ? q : 2 * q + (i >> 2)][i & 3];
+        if (ws) {
+            float *o = ws + m * p.N + n;
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                if (n + i + 4 <= p.N) {
+                    *reinterpret_cast<lcf_f4u *>(o + i) = (lcf_f4u){v[i], v[i + 1], v[i + 2], v[i + 3]};
+                } else {
+#pragma unroll
+                    for (int k = i; k < i + 4; ++k)
+                        if (n + k < p.N) o[k] = v[k];
+                }
+            }
+        } else if (n < p.N) {
+            f8_store<W>(p, m, n, v, p.N - n);
+        }
     }
 }
 
@@ -298,52 +366,71 @@ template <int F> __device__ __forceinline__ f8_b8 f8_to_bf16(int lo, int hi, flo
     return v;
 }
 
-// One workgroup of four waves makes BM x BN outputs, a wave BM/2 x BN/2 of them (WN = BN/2 = 64).
-// The instruction's first operand is b, its second a: a lane then holds four consecutive columns n
-// of one row m for each 16 x 16 piece, and with the pieces' rows dealt as n = 16 g + 4 t + r
-// (g = lane / 16, t = piece, r = register) sixteen consecutive columns over the four pieces of a
-// wave: whole 128-byte lines of a bf16 output leave straight from the registers.
-// LDS holds 128 bytes of k for each row of a and b, twice (the next step's loads are in flight
-// while this one multiplies).  A 16-byte piece c of row r sits at place c ^ swz(r), so that the
-// eight lanes of a bank group read eight different places.
-template <int FA, int FB, bool WIDE, int BM>
-__global__ void __launch_bounds__(256) f8_gemm_kernel(F8Gemm p)
+// A workgroup of WM x WN waves makes BM x BN outputs, a wave 16 MT x 64 of them.
+// LDS holds 128 bytes of k for each row of a and b, twice: the next step's bytes go from memory
+// straight into LDS (16 bytes a lane, no registers) while this one multiplies.  A 16-byte piece c of
+// row r sits at place c ^ swz(r), so that the lanes that read together read different banks; a
+// memory-to-LDS load writes its 64 lanes' pieces side by side, so it is the lanes' addresses in
+// memory that are dealt.  Rows past the end are read as the last row, and what lies behind K is cut
+// from the registers in the last step.
+template <int FA, int FB, bool WIDE, int WM, int WN, int MT>
+__global__ void __launch_bounds__(WM *WN * 64) f8_gemm_kernel(F8Gemm p)
 {
-    constexpr int BN = 128, MT = BM / 32; // MT: 16-row pieces of a wave
+    constexpr int BM = WM * MT * 16, BN = WN * 64, NT = WM * WN * 64;
+    constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT; // 16-byte pieces a thread loads for a step
     extern __shared__ __align__(16) unsigned char smem[];
-    // a: [2][BM][128], b: [2][BN][128]
-    unsigned char *la = smem, *lb = smem + 2 * BM * 128;
+    // a: [2][BM][128], b: [2][BN][128], scale words: [2][BM + BN]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r16 = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x;
-    const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+    // workgroups go round-robin to the 8 XCDs: XCD x takes the x-th eighth of the tiles, in groups
+    // of 8 tile rows, so that the tiles in flight on it share rows of a and b in its L2
+    // (the splits of a long sum come one after the other)
+    const int tiles = p.tiles_m * p.tiles_n, per = (tiles * p.splits + 7) >> 3;
+    const int all = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || all >= tiles * p.splits) return;
+    const int split = all / tiles, lin = all - split * tiles;
+    const int band = lin / (8 * p.tiles_n), first = band * 8;
+    const int high = min(8, p.tiles_m - first), in = lin - band * 8 * p.tiles_n;
+    const int tm = first + in % high, tn = in / high;
     const int m0 = tm * BM, n0 = tn * BN;
-    const int wm = (wave & 1) * (BM / 2), wn = (wave >> 1) * 64;
-    const int steps_all = (p.K + 127) >> 7;
-    const int step0 = blockIdx.y * p.ksteps;
-    const int step1 = min(steps_all, step0 + p.ksteps);
+    const int wm = (wave % WM) * (MT * 16), wn = (wave / WM) * 64;
+    const int step0 = split * p.ksteps;
+    const int step1 = min((p.K + 127) >> 7, step0 + p.ksteps);
 
     auto swz_a = [](int r) { return r & 7; };
-    auto swz_b = [](int r) { return (r & 3) | ((r >> 2) & 4); }; // rows 16 apart take the other half
+    // a fragment's rows of b are f8_column(t, 0..15): their bits 0..2, or 0, 1 and 3, tell eight apart
+    auto swz_b = [](int r) { return WIDE ? r & 7 : (r & 3) | ((r >> 1) & 4); };
 
-    auto load = [&](int buf, int step) {
+    // this thread's pieces, as offsets from the tile's first row (ld <= 2^22: 32 bits) into buffers
+    // that end with the last row's last piece: past it a load brings zeros and touches nothing
+    const int rows_a = min(BM, p.M - m0), rows_b = min(BN, p.N - n0), room = (p.K + 15) & ~15;
+    const __amdgpu_buffer_rsrc_t abuf = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char *>(p.a + (long long)m0 * p.lda), 0, (rows_a - 1) * (int)p.lda + room, 0x00020000);
+    const __amdgpu_buffer_rsrc_t bbuf = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char *>(p.b + (long long)n0 * p.ldb), 0, (rows_b - 1) * (int)p.ldb + room, 0x00020000);
+    int aoff[LA], boff[LB];
+    static_assert((NT >> 3) % 32 == 0, "a thread's pieces have one column");
+    {
+        const int r = tid >> 3;
 #pragma unroll
-        for (int i = 0; i < BM / 32; ++i) {
-            const int slot = i * 256 + tid, r = slot >> 3, c = (slot & 7) ^ swz_a(r);
-            const int row = min(m0 + r, p.M - 1);
-            int col = step * 128 + c * 16;
-            if (col >= p.K) col = 0; // read, but cut away below
-            *reinterpret_cast<uint4 *>(la + buf * BM * 128 + slot * 16) =
-                *reinterpret_cast<const uint4 *>(p.a + row * p.lda + col);
+        for (int i = 0; i < LA; ++i)
+            aoff[i] = min(i * (NT >> 3) + r, rows_a - 1) * (int)p.lda + (((tid & 7) ^ swz_a(r)) + step0 * 8) * 16;
+#pragma unroll
+        for (int i = 0; i < LB; ++i)
+            boff[i] = min(i * (NT >> 3) + r, rows_b - 1) * (int)p.ldb + (((tid & 7) ^ swz_b(r)) + step0 * 8) * 16;
+    }
+    // the next step in turn: 128 bytes further each time
+    auto load = [&](int buf) {
+        unsigned char *la = smem + buf * BM * 128 + wave * 1024, *lb = smem + 2 * BM * 128 + buf * BN * 128 + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < LA; ++i) {
+            f8_lds16(abuf, la + i * NT * 16, aoff[i]);
+            aoff[i] += 128;
         }
 #pragma unroll
-        for (int i = 0; i < BN / 32; ++i) {
-            const int slot = i * 256 + tid, r = slot >> 3, c = (slot & 7) ^ swz_b(r);
-            const int row = min(n0 + r, p.N - 1);
-            int col = step * 128 + c * 16;
-            if (col >= p.K) col = 0;
-            *reinterpret_cast<uint4 *>(lb + buf * BN * 128 + slot * 16) =
-                *reinterpret_cast<const uint4 *>(p.b + row * p.ldb + col);
+        for (int i = 0; i < LB; ++i) {
+            f8_lds16(bbuf, lb + i * NT * 16, boff[i]);
+            boff[i] += 128;
         }
     };
 
@@ -352,138 +439,342 @@ __global__ void __launch_bounds__(256) f8_gemm_kernel(F8Gemm p)
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[i][t] = (f8_f4){0.f, 0.f, 0.f, 0.f};
-    int rowa[MT], rowb[4];   // LDS rows of this lane's pieces
-    const unsigned *sap[MT]; // their scales, four steps to a word
-    const unsigned *sbp[4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        rowa[i] = wm + i * 16 + r16;
-        sap[i] = (const unsigned *)(p.sa + (long long)min(m0 + rowa[i], p.M - 1) * p.ldsa);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        rowb[t] = wn + (r16 >> 2) * 16 + t * 4 + (r16 & 3);
-        sbp[t] = (const unsigned *)(p.sb + (long long)(min(n0 + rowb[t], p.N - 1) >> p.b_shift) * p.ldsb);
-    }
-    if (step0 < step1) load(0, step0);
-    __syncthreads();
-    for (int step = step0; step < step1; ++step) {
-        const int buf = (step - step0) & 1;
-        if (step + 1 < step1) load(buf ^ 1, step + 1);
-        int xa[MT], xb[4];
+    const int nb = f8_column<WIDE>(0, r16); // this lane's row of b in piece 0 of the wave
+    // scale words, four steps to a word, go through LDS as well: one word a thread (there are as many
+    // threads as rows of a and b), twice
+    static_assert(NT == BM + BN, "a thread for each row's scales");
+    unsigned *ls = (unsigned *)(smem + 2 * (BM + BN) * 128);
+    const unsigned char *srow =
+        tid < BM ? p.sa + (long long)min(m0 + tid, p.M - 1) * p.ldsa
+                 : p.sb + (long long)(min(n0 + tid - BM, p.N - 1) >> p.b_shift) * p.ldsb;
+    auto load_scales = [&](int word) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(srow + word * 4),
+                                         (__attribute__((address_space(3))) void *)(ls + (word & 1) * NT + wave * 64),
+                                         4, 0, 0);
+    };
+    unsigned xa[MT], xb[4];
+    auto scales = [&](int step) {
+        const unsigned *l = ls + ((step >> 2) & 1) * NT;
         const int sh = (step & 3) * 8;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) xa[i] = sap[i][step >> 2] >> sh;
+        for (int i = 0; i < MT; ++i) xa[i] = l[wm + i * 16 + r16] >> sh;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) xb[t] = sbp[t][step >> 2] >> sh;
-        const bool tail = step * 128 + 128 > p.K;
-        auto frag = [&](const unsigned char *base, int r, int s) -> f8_v8 {
-            f8_v8 v;
-            const f8_v4 lo = *reinterpret_cast<const f8_v4 *>(base + r * 128 + ((g ^ s) * 16));
-            const f8_v4 hi = *reinterpret_cast<const f8_v4 *>(base + r * 128 + (((g + 4) ^ s) * 16));
+        for (int t = 0; t < 4; ++t) xb[t] = l[BM + wn + f8_column<WIDE>(t, r16)] >> sh;
+    };
+
+    auto multiply = [&](int buf, int step, auto tail) {
+        const unsigned char *la = smem + buf * BM * 128 + (wm + r16) * 128;
+        const unsigned char *lb = smem + 2 * BM * 128 + buf * BN * 128 + (wn + nb) * 128;
+        const int sa = swz_a(r16), sb0 = swz_b(wn + nb);
+        auto frag = [&](const unsigned char *row, int s) -> f8_v8 {
+            const f8_v4 lo = *reinterpret_cast<const f8_v4 *>(row + ((g ^ s) * 16));
+            const f8_v4 hi = *reinterpret_cast<const f8_v4 *>(row + (((g + 4) ^ s) * 16));
             int w[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (tail) {
+            if constexpr (decltype(tail)::value) {
                 f8_cut(w, step * 128 + g * 16, p.K);
                 f8_cut(w + 4, step * 128 + g * 16 + 64, p.K);
             }
+            f8_v8 v;
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = w[i];
             return v;
         };
-        f8_v8 fb[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) fb[t] = frag(lb + buf * BN * 128, rowb[t], swz_b(rowb[t]));
         if constexpr (!WIDE) {
+            f8_v8 fb[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) fb[t] = frag(lb + f8_column<WIDE>(t, 0) * 128, sb0);
+            // the next piece of a is on its way while this one multiplies; the scheduler is kept from
+            // reading all of them first, which would cost more registers than there are
+            f8_v8 fa = frag(la, sa);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const f8_v8 fa = frag(la + buf * BM * 128, rowa[i], swz_a(rowa[i]));
+                f8_v8 next = fa;
+                if (i + 1 < MT) next = frag(la + (i + 1) * 2048, sa);
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
                     acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[t], fa, acc[i][t], FB, FA, 0,
-                                                                                 xb[t], 0, xa[i]);
+                                                                                 (int)xb[t], 0, (int)xa[i]);
+                fa = next;
+                if constexpr (!decltype(tail)::value) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
             f8_b8 wb[4][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < 4; ++t) {
+                const f8_v8 fb = frag(lb + f8_column<WIDE>(t, 0) * 128, sb0);
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
-                    wb[t][s] = f8_to_bf16<FB>(fb[t][2 * s], fb[t][2 * s + 1], lcf_exp2i((xb[t] & 255) - 127));
+                    wb[t][s] = f8_to_bf16<FB>(fb[2 * s], fb[2 * s + 1], lcf_exp2i((int)(xb[t] & 255) - 127));
+            }
+            f8_v8 fa = frag(la, sa);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const f8_v8 fa = frag(la + buf * BM * 128, rowa[i], swz_a(rowa[i]));
+                f8_v8 next = fa;
+                if (i + 1 < MT) next = frag(la + (i + 1) * 2048, sa);
+                const float ea = lcf_exp2i((int)(xa[i] & 255) - 127);
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    const f8_b8 wa = f8_to_bf16<FA>(fa[2 * s], fa[2 * s + 1], lcf_exp2i((xa[i] & 255) - 127));
+                    const f8_b8 wa = f8_to_bf16<FA>(fa[2 * s], fa[2 * s + 1], ea);
 #pragma unroll
                     for (int t = 0; t < 4; ++t)
                         acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[t][s], wa, acc[i][t], 0, 0, 0);
                 }
+                fa = next;
+                if constexpr (!decltype(tail)::value) __builtin_amdgcn_sched_barrier(0);
             }
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xa[i] >>= 8;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) xb[t] >>= 8;
+    };
+
+    if (step0 < step1) {
+        load_scales(step0 >> 2);
+        load(0);
         __syncthreads();
+        const int whole = min(step1, p.K >> 7); // steps that K does not end in
+        int step = step0;
+        // nothing but the barrier may follow the products in the loop: behind a branch the compiler
+        // would move them past the barrier, and the loads would have nothing to hide behind
+#pragma clang loop unroll(disable)
+        for (; step < whole; ++step) {
+            const int buf = (step - step0) & 1;
+            if (step + 1 < step1) {
+                if (((step + 1) & 3) == 0) load_scales((step + 1) >> 2);
+                load(buf ^ 1);
+            }
+            if (step == step0 || (step & 3) == 0) scales(step);
+            multiply(buf, step, F8Bool<false>());
+            __syncthreads();
+        }
+        if (step < step1 && (step == step0 || (step & 3) == 0)) scales(step);
+        if (step < step1) multiply((step - step0) & 1, step, F8Bool<true>());
     }
-    const int n = n0 + wn + g * 16;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) f8_pin(acc[i]);
+    float *ws = p.ws ? p.ws + (long long)split * p.M * p.N : nullptr;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const long long m = m0 + wm + i * 16 + r16;
-        if (m >= p.M || n >= p.N) continue;
-        float v[16];
+        if (m < p.M) f8_put<WIDE>(p, ws, m, n0 + wn, g, acc[i]);
+    }
+}
+
+// Thin layers (K <= 512, N <= 256) over many rows: bound by reading a and writing out.  A wave keeps
+// its 64 columns of b (all of K: 32 KS registers, 64 KS widened) and walks down the rows, 16 at a
+// time, straight from memory to the matrix core and back: nothing goes through LDS and nothing
+// waits for another wave.  The waves of a workgroup that share rows read them through the same L1.
+// The next 16 rows are asked for before this one's are used.  Their loads stand behind no branch
+// (a load behind one would make every later wait assume the worst): what lies past the last row or
+// past K is an offset beyond the buffer's end, which brings zeros and touches no memory.
+// T: the rows are fp32 / bf16 / fp16 and brought into 8-bit form in registers on the way (bit for
+// bit what f8_rows_kernel stores: a row's 128 columns are in the four lanes of equal r16), which
+// saves writing and reading them; T = unsigned char: they are in that form already.
+template <int FA, int FB, bool WIDE, int KS, typename T>
+__global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
+{
+    constexpr int E = sizeof(T), P = 2 * E; // 16-byte pieces of a row for one step of 128 columns, a lane
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int n0 = (wave & ((1 << wn_shift) - 1)) * 64;
+    if (n0 >= p.N) return;
+    const int rows = 16 << (2 - wn_shift), wm = (wave >> wn_shift) * 16; // rows a workgroup takes at a time
+
+    f8_v8 fb[KS][4];
+    unsigned xb[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t) {
+        const int n = min(n0 + f8_column<WIDE>(t, r16), p.N - 1);
+        xb[t] = *(const unsigned *)(p.sb + (long long)(n >> p.b_shift) * p.ldsb);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[t * 4 + r] = acc[i][t][r];
-        if (p.ws) {
-            float *o = p.ws + ((long long)blockIdx.y * p.M + m) * p.N + n;
-            if (n + 16 <= p.N) {
-                lcf_st8(o, v);
-                lcf_st8(o + 8, v + 8);
-            } else {
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    if (n + k < p.N) o[k] = v[k];
+            for (int h = 0; h < 2; ++h) {
+                const int col = k * 128 + g * 16 + h * 64;
+                f8_v4 v = (f8_v4){0, 0, 0, 0};
+                if (col < p.K) v = *reinterpret_cast<const f8_v4 *>(p.b + (long long)n * p.ldb + col);
+                int w[4] = {v[0], v[1], v[2], v[3]};
+                f8_cut(w, col, p.K);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) fb[k][t][h * 4 + i] = w[i];
+            }
+    }
+    f8_b8 wb[WIDE ? KS : 1][4][4];
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    wb[k][t][q] = f8_to_bf16<FB>(fb[k][t][2 * q], fb[k][t][2 * q + 1],
+                                                 lcf_exp2i((int)((xb[t] >> (8 * k)) & 255) - 127));
+    }
+
+    // piece i of step k holds elements col .. col + 16 / E of the row: the lane's 16 columns from
+    // 16 g on, then the 16 from 64 + 16 g on
+    struct Rows {
+        f8_v4 v[KS * P];
+        unsigned s;
+    };
+    int off[KS * P];
+    const int room = E == 1 ? (p.K + 15) & ~15 : p.K;
+#pragma unroll
+    for (int i = 0; i < KS * P; ++i) {
+        const int h = i % P, col = (i / P) * 128 + (h / (P / 2)) * 64 + g * 16 + (h % (P / 2)) * (16 / E);
+        off[i] = col < p.K ? (r16 * (int)p.lda + col) * E : (int)0x80000000;
+    }
+    auto ask = [&](long long m0, Rows &x) {
+        const int left = (int)(m0 < p.M ? (p.M - m0 < 16 ? p.M - m0 : 16) : 0);
+        const __amdgpu_buffer_rsrc_t buf = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<unsigned char *>(p.a + (left ? m0 * p.lda * E : 0)), 0,
+            left ? ((left - 1) * (int)p.lda + room) * E : 0, 0x00020000);
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < KS * P; ++i) {
+            const u4 v = __builtin_amdgcn_raw_buffer_load_b128(buf, off[i], 0, 0);
+            x.v[i] = (f8_v4){(int)v[0], (int)v[1], (int)v[2], (int)v[3]};
+        }
+        if constexpr (E == 1) {
+            const long long m = m0 + r16 < p.M ? m0 + r16 : p.M - 1;
+            x.s = *(const unsigned *)(p.sa + m * p.ldsa);
+        }
+    };
+    auto use = [&](long long m0, const Rows &x) {
+        int fa[KS][8];
+        unsigned xa = 0;
+        if constexpr (E == 1) {
+            xa = x.s;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) fa[k][i] = x.v[k * 2 + (i >> 2)][i & 3];
+                if (p.K & 15) {
+                    f8_cut(fa[k], k * 128 + g * 16, p.K);
+                    f8_cut(fa[k] + 4, k * 128 + g * 16 + 64, p.K);
+                }
             }
         } else {
-            f8_store(p, m, n, v, p.N - n);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int w = x.v[k * P + i * E / 16][(i * E / 4) & 3];
+                    if constexpr (E == 4) v[i] = __int_as_float(w);
+                    else v[i] = lcf_to_f32(__builtin_bit_cast(T, (unsigned short)((unsigned)w >> (16 * (i & 1)))));
+                }
+                float top = lcf_f8_top<32>(v);
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const int e = lcf_f8_exponent(top, FA);
+                const float sc = lcf_exp2i(-e);
+                xa |= (unsigned)(e + 127) << (8 * k);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    fa[k][i] = (int)lcf_f8_pack4(v[4 * i] * sc, v[4 * i + 1] * sc, v[4 * i + 2] * sc, v[4 * i + 3] * sc,
+                                                 FA);
+            }
         }
+        f8_f4 acc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = (f8_f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if constexpr (WIDE) {
+                const float ea = lcf_exp2i((int)((xa >> (8 * k)) & 255) - 127);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f8_b8 wa = f8_to_bf16<FA>(fa[k][2 * q], fa[k][2 * q + 1], ea);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[k][t][q], wa, acc[t], 0, 0, 0);
+                }
+            } else {
+                f8_v8 a;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = fa[k][i];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        fb[k][t], a, acc[t], FB, FA, 0, (int)(xb[t] >> (8 * k)), 0, (int)(xa >> (8 * k)));
+            }
+        }
+        f8_pin(acc);
+        if (m0 + r16 < p.M) f8_put<WIDE>(p, nullptr, m0 + r16, n0, g, acc);
+    };
+    const long long stride = (long long)gridDim.x * rows;
+    long long m0 = (long long)blockIdx.x * rows + wm;
+    Rows x, next;
+    ask(m0, x);
+    for (; m0 < p.M; m0 += stride) {
+        ask(m0 + stride, next);
+        use(m0, x);
+        x = next;
     }
 }
 
-// joins the splits' parts in their order and applies the epilogue; 16 columns a thread
+// joins the splits' parts in a fixed order and applies the epilogue.  A workgroup takes 64
+// consecutive elements: thread = (split line t / 16, four elements t % 16); 16 lines run over the
+// splits side by side and meet in LDS.
 __global__ void __launch_bounds__(256) f8_join_kernel(F8Gemm p, int splits)
 {
-    const int per = (p.N + 15) >> 4;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)p.M * per) return;
-    const long long m = i / per;
-    const int n = (int)(i - m * per) * 16, count = p.N - n;
-    float v[16];
+    __shared__ float lds[16][64];
+    const long long total = (long long)p.M * p.N;
+    const int part = threadIdx.x & 15, line = threadIdx.x >> 4;
+    const long long e = (long long)blockIdx.x * 64 + part * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = line; s < splits; s += 16) {
+        const float *o = p.ws + s * total + e;
+        if (e + 4 <= total) {
+            const lcf_f4u q = *reinterpret_cast<const lcf_f4u *>(o);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float *o = p.ws + ((long long)s * p.M + m) * p.N + n;
+            for (int k = 0; k < 4; ++k) v[k] += q[k];
+        } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (k < count) v[k] += o[k];
+            for (int k = 0; k < 4; ++k)
+                if (e + k < total) v[k] += o[k];
+        }
     }
-    f8_store(p, m, n, v, count);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) lds[line][part * 4 + k] = v[k];
+    __syncthreads();
+    const long long i = (long long)blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x >= 64 || i >= total) return;
+    float x = 0.f;
+#pragma unroll
+    for (int l = 0; l < 16; ++l) x += lds[l][threadIdx.x];
+    const long long m = i / p.N;
+    const int n = (int)(i - m * p.N);
+    if (p.scale) x *= p.scale[n];
+    if (p.shift) x += p.shift[n];
+    if (p.relu) x = x < 0.f ? 0.f : x;
+    if (p.code == LCF_F32) ((float *)p.out)[m * p.ldo + n] = x;
+    else if (p.code == LCF_BF16) ((lcf_b *)p.out)[m * p.ldo + n] = lcf_from_f32<lcf_b>(x);
+    else ((lcf_h *)p.out)[m * p.ldo + n] = lcf_from_f32<lcf_h>(x);
 }
 
+static bool f8_is_thin(int M, int N, int K, bool wide);
 struct F8Plan {
-    int bm, tiles_m, tiles_n, splits, ksteps;
+    int thin, big, tiles_m, tiles_n, splits, ksteps;
 };
-static F8Plan f8_plan(int M, int N, int K)
+static F8Plan f8_plan(int M, int N, int K, bool wide)
 {
     F8Plan q;
-    q.bm = 128;
-    q.tiles_m = (M + 127) / 128;
-    q.tiles_n = (N + 127) / 128;
+    q.thin = f8_is_thin(M, N, K, wide);
+    const long long t256 = (long long)((M + 255) / 256) * ((N + 255) / 256);
+    q.big = t256 >= 192;
+    const int bm = q.big ? 256 : 128;
+    q.tiles_m = (M + bm - 1) / bm;
+    q.tiles_n = (N + bm - 1) / bm;
     const int steps = (K + 127) / 128;
     const long long tiles = (long long)q.tiles_m * q.tiles_n;
     // a few tiles over a long sum: split it until the chip's 256 units have work, at least four
     // steps to a split
     int splits = 1;
-    if (tiles < 128) {
+    if (!q.thin && tiles < 128) {
         splits = (int)(256 / tiles);
         if (splits > steps / 4) splits = steps / 4;
         if (splits < 1) splits = 1;
@@ -494,18 +785,91 @@ static F8Plan f8_plan(int M, int N, int K)
     return q;
 }
 
-extern "C" size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K)
+extern "C" size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype)
 {
     if (M < 1 || N < 1 || K < 1) return 0;
-    const F8Plan q = f8_plan(M, N, K);
+    const F8Plan q = f8_plan(M, N, K, out_dtype == LCF_F32);
     return q.splits > 1 ? (size_t)q.splits * M * N * sizeof(float) : 0;
 }
 
-template <int FA, int FB> static void f8_gemm_launch(const F8Gemm &p, const F8Plan &q, hipStream_t st)
+// whether f8_stream_kernel takes a product: b in registers, and rows enough for every wave
+static bool f8_is_thin(int M, int N, int K, bool wide)
 {
-    const dim3 grid(q.tiles_m * q.tiles_n, q.splits);
-    if (p.code == LCF_F32) f8_gemm_kernel<FA, FB, true, 128><<<grid, 256, 2 * (128 + 128) * 128, st>>>(p);
-    else f8_gemm_kernel<FA, FB, false, 128><<<grid, 256, 2 * (128 + 128) * 128, st>>>(p);
+    return K > 0 && K <= (wide ? 256 : 512) && N <= 256 && M >= 4096;
+}
+
+template <int FA, int FB, bool WIDE, typename T> static int f8_stream_launch(const F8Gemm &p, hipStream_t st)
+{
+    const int wn_shift = p.N <= 64 ? 0 : p.N <= 128 ? 1 : 2, rows = 16 << (2 - wn_shift);
+    const long long want = ((long long)p.M + rows - 1) / rows;
+    // as many workgroups as the chip holds at once (by the registers they need)
+    const int ks = (p.K + 127) / 128, most = 256 * (WIDE ? (ks == 1 ? 3 : 2) : ks == 1 ? 5 : ks == 2 ? 3 : 2);
+    const int grid = (int)(want < most ? want : most);
+    if (ks == 1) f8_stream_kernel<FA, FB, WIDE, 1, T><<<grid, 256, 0, st>>>(p, wn_shift);
+    else if (ks == 2) f8_stream_kernel<FA, FB, WIDE, 2, T><<<grid, 256, 0, st>>>(p, wn_shift);
+    else if constexpr (!WIDE) f8_stream_kernel<FA, FB, WIDE, 4, T><<<grid, 256, 0, st>>>(p, wn_shift);
+    LCF_CHECK_LAUNCH();
+    return LCF_OK;
+}
+
+template <int FA, int FB, bool WIDE> static int f8_gemm_launch2(const F8Gemm &p, const F8Plan &q, hipStream_t st)
+{
+    if (q.thin) return f8_stream_launch<FA, FB, WIDE, unsigned char>(p, st);
+    const unsigned grid = (unsigned)(((long long)q.tiles_m * q.tiles_n * q.splits + 7) / 8 * 8);
+    // more LDS than a launch may take unasked
+    if (q.big) {
+        const void *f = (const void *)f8_gemm_kernel<FA, FB, WIDE, 2, 4, 8>;
+        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 512 * 132) != hipSuccess)
+            return LCF_ERR_LAUNCH;
+        f8_gemm_kernel<FA, FB, WIDE, 2, 4, 8><<<grid, 512, 2 * 512 * 132, st>>>(p);
+    } else {
+        const void *f = (const void *)f8_gemm_kernel<FA, FB, WIDE, 2, 2, 4>;
+        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 256 * 132) != hipSuccess)
+            return LCF_ERR_LAUNCH;
+        f8_gemm_kernel<FA, FB, WIDE, 2, 2, 4><<<grid, 256, 2 * 256 * 132, st>>>(p);
+    }
+    LCF_CHECK_LAUNCH();
+    return LCF_OK;
+}
+template <int FA, int FB> static int f8_gemm_launch(const F8Gemm &p, const F8Plan &q, hipStream_t st)
+{
+    return p.code == LCF_F32 ? f8_gemm_launch2<FA, FB, true>(p, q, st) : f8_gemm_launch2<FA, FB, false>(p, q, st);
+}
+
+// x [M, K] of fp32 / bf16 / fp16 rows through b [N, K] in one launch
+extern "C" int lcf_f8_linear(const void *x, long long ldx, int dtype, const void *b, long long ldb,
+                             const unsigned char *sb, int ldsb, int b_square, int M, int N, int K, const float *scale,
+                             const float *shift, int relu, void *out, long long ldo, int out_dtype, void *stream)
+{
+    if (M < 0 || N < 0 || K < 0 || !lcf_is_type(dtype) || !lcf_is_type(out_dtype)) return LCF_ERR_ARG;
+    if (M == 0 || N == 0) return LCF_OK;
+    if (!out || ldo < N) return LCF_ERR_ARG;
+    if (K > 0 && (!x || ldx < K || !f8_form_ok(b, ldb, sb, ldsb, K))) return LCF_ERR_ARG;
+    // rows are read 16 bytes at a time, by buffer loads that want four-byte addresses
+    if (!f8_is_thin(M, N, K, out_dtype == LCF_F32) || dtype != out_dtype || (K & 7) || ((uintptr_t)x & 3) ||
+        (ldx * lcf_type_size(dtype) & 3) || ldx > (1 << 22) || ldb > (1 << 22))
+        return LCF_ERR_UNSUPPORTED;
+    F8Gemm p{};
+    p.a = (const unsigned char *)x;
+    p.lda = ldx;
+    p.b = (const unsigned char *)b;
+    p.ldb = ldb;
+    p.sb = sb;
+    p.ldsb = ldsb;
+    p.b_shift = b_square ? 7 : 0;
+    p.scale = scale;
+    p.shift = shift;
+    p.relu = relu;
+    p.out = out;
+    p.ldo = ldo;
+    p.code = out_dtype;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == LCF_F32) return f8_stream_launch<0, 0, true, float>(p, st);
+    if (dtype == LCF_BF16) return f8_stream_launch<0, 0, false, lcf_b>(p, st);
+    return f8_stream_launch<0, 0, false, lcf_h>(p, st);
 }
 
 extern "C" int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa, int ldsa, int a_fmt, const void *b,
@@ -518,24 +882,26 @@ extern "C" int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa
     if (M == 0 || N == 0) return LCF_OK;
     if (!out || ldo < N) return LCF_ERR_ARG;
     if (K > 0 && (!f8_form_ok(a, lda, sa, ldsa, K) || !f8_form_ok(b, ldb, sb, ldsb, K))) return LCF_ERR_ARG;
-    const F8Plan q = f8_plan(M, N, K);
-    if ((long long)q.tiles_m * q.tiles_n > 0x7FFFFFFFll) return LCF_ERR_UNSUPPORTED;
+    const F8Plan q = f8_plan(M, N, K, out_dtype == LCF_F32);
+    // tiles are counted, and a tile's rows addressed, in 32 bits
+    if ((long long)q.tiles_m * q.tiles_n * q.splits > 0x7FFFFF00ll || lda > (1 << 22) || ldb > (1 << 22))
+        return LCF_ERR_UNSUPPORTED;
     if (q.splits > 1) {
         if (!ws) return LCF_ERR_ARG;
         if (ws_bytes < (size_t)q.splits * M * N * sizeof(float)) return LCF_ERR_WORKSPACE;
     }
     F8Gemm p{(const unsigned char *)a, sa, (const unsigned char *)b, sb, scale, shift, out,
              q.splits > 1 ? (float *)ws : nullptr, lda, ldb, ldo, ldsa, ldsb, b_square ? 7 : 0, M, N, K, relu,
-             out_dtype, q.tiles_m, q.tiles_n, q.ksteps};
+             out_dtype, q.tiles_m, q.tiles_n, q.splits, q.ksteps};
     hipStream_t st = (hipStream_t)stream;
-    if (a_fmt == LCF_E4M3 && b_fmt == LCF_E4M3) f8_gemm_launch<0, 0>(p, q, st);
-    else if (a_fmt == LCF_E4M3) f8_gemm_launch<0, 1>(p, q, st);
-    else if (b_fmt == LCF_E4M3) f8_gemm_launch<1, 0>(p, q, st);
-    else f8_gemm_launch<1, 1>(p, q, st);
-    LCF_CHECK_LAUNCH();
+    int rc;
+    if (a_fmt == LCF_E4M3 && b_fmt == LCF_E4M3) rc = f8_gemm_launch<0, 0>(p, q, st);
+    else if (a_fmt == LCF_E4M3) rc = f8_gemm_launch<0, 1>(p, q, st);
+    else if (b_fmt == LCF_E4M3) rc = f8_gemm_launch<1, 0>(p, q, st);
+    else rc = f8_gemm_launch<1, 1>(p, q, st);
+    if (rc != LCF_OK) return rc;
     if (q.splits > 1) {
-        const long long n = (long long)M * ((N + 15) / 16);
-        f8_join_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, q.splits);
+        f8_join_kernel<<<(unsigned)(((long long)M * N + 63) / 64), 256, 0, st>>>(p, q.splits);
         LCF_CHECK_LAUNCH();
     }
     return LCF_OK;

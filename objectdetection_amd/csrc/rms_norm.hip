@@ -99,12 +99,12 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) rn_fwd_kernel(RnFwd p)
             for (int i = 0; i < 8; ++i) h[c][i] = h[c][i] * inv * w[c][i];
             if (live && p.y && col < p.width) lcf_st8_tail((T *)p.y + row * p.width, col, p.width, h[c]);
             if (p.q8) {
-                float top = 0.f;
+                if (col + 8 > p.width) { // an infinite inv makes NaN behind the row
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (col + i >= p.width) h[c][i] = 0.f; // an infinite inv makes NaN behind the row
-                    top = fmaxf(top, lcf_finite_abs(h[c][i]));
+                    for (int i = 0; i < 8; ++i)
+                        if (col + i >= p.width) h[c][i] = 0.f;
                 }
+                float top = lcf_f8_top<8>(h[c]);
 #pragma unroll
                 for (int d = (LPR < 16 ? LPR : 16) / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
                 const int e = lcf_f8_exponent(top, p.fmt);
@@ -217,22 +217,45 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) rn_bwd_kernel(RnBwd p)
     }
 }
 
-// dweight [width] = sum of the workgroups' parts, in 64 bits: 32 columns x 8 lines a workgroup
-__global__ void __launch_bounds__(256)
+// dweight [width] = sum of the workgroups' parts, in 64 bits and in a fixed order.  A workgroup
+// takes 16 columns: thread = (part line t / 4, four columns t % 4), 256 lines, so that a thread has
+// four loads in flight and no chain of them (one line per wave took 32 us for 1024 parts).
+__global__ void __launch_bounds__(1024)
 rn_dweight_kernel(const float *__restrict__ parts, int nparts, int width, void *__restrict__ dw, int code)
 {
-    __shared__ double lds[8][32];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), line = threadIdx.x >> 5;
-    double s = 0.0;
-    if (col < width)
-        for (int i = line; i < nparts; i += 8) s += (double)parts[(size_t)i * width + col];
-    lds[line][threadIdx.x & 31] = s;
+    __shared__ double lds[16][16];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 3) * 4, line = threadIdx.x >> 2;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+    for (int i = line; i < nparts; i += 256) {
+        const float *q = parts + (size_t)i * width + col;
+        if (col + 4 <= width) {
+            const lcf_f4u v = *reinterpret_cast<const lcf_f4u *>(q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += (double)v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < width) s[j] += (double)q[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int d = 32; d >= 4; d >>= 1) s[j] += __shfl_xor(s[j], d, 64);
+    }
+    if ((threadIdx.x & 63) < 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lds[threadIdx.x >> 6][(threadIdx.x & 3) * 4 + j] = s[j];
+    }
     __syncthreads();
-    if (line == 0 && col < width) {
-        for (int i = 1; i < 8; ++i) s += lds[i][threadIdx.x];
-        if (code == LCF_F32) ((float *)dw)[col] = (float)s;
-        else if (code == LCF_BF16) ((lcf_b *)dw)[col] = (lcf_b)(float)s;
-        else ((lcf_h *)dw)[col] = (lcf_h)(float)s;
+    const int c = blockIdx.x * 16 + threadIdx.x;
+    if (threadIdx.x < 16 && c < width) {
+        double t = 0.0;
+        for (int i = 0; i < 16; ++i) t += lds[i][threadIdx.x];
+        if (code == LCF_F32) ((float *)dw)[c] = (float)t;
+        else if (code == LCF_BF16) ((lcf_b *)dw)[c] = lcf_from_f32<lcf_b>((float)t);
+        else ((lcf_h *)dw)[c] = lcf_from_f32<lcf_h>((float)t);
     }
 }
 
@@ -331,7 +354,7 @@ extern "C" int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, lo
         LCF_CHECK_LAUNCH();
     }
     if (dweight) {
-        rn_dweight_kernel<<<(width + 31) / 32, 256, 0, st>>>((const float *)ws, grid, width, dweight, weight_dtype);
+        rn_dweight_kernel<<<(width + 15) / 16, 1024, 0, st>>>((const float *)ws, grid, width, dweight, weight_dtype);
         LCF_CHECK_LAUNCH();
     }
     return LCF_OK;

@@ -113,22 +113,28 @@ __device__ __forceinline__ int lcf_f8_exponent(float amax, int fmt)
 }
 __device__ __forceinline__ float lcf_exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-// |v| where v is finite, else 0: what a block's largest magnitude is taken over
-__device__ __forceinline__ float lcf_finite_abs(float v)
+// Largest magnitude of N values of a lane, NaN left out (fmax does that by itself).  Infinities do
+// not enter a block's scale either, and e4m3 holds none: only where one is found, anywhere in the
+// wave (a uniform branch), they are made NaN in place and the others looked through again.
+template <int N> __device__ __forceinline__ float lcf_f8_top(float *v)
 {
-    const float a = __builtin_fabsf(v);
-    return a <= 3.402823466e38f ? a : 0.f;
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, __builtin_fabsf(v[i]));
+    if (__builtin_expect(__any(top > 3.402823466e38f), 0)) {
+        top = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (__builtin_fabsf(v[i]) > 3.402823466e38f) v[i] = __uint_as_float(0x7FC00000u);
+            top = fmaxf(top, __builtin_fabsf(v[i]));
+        }
+    }
+    return top;
 }
 
-// four values, already scaled, to four bytes.  Infinities and NaN become NaN: e4m3 holds no
-// infinity, and what the conversion makes of one would depend on the overflow mode.
+// four values, already scaled (finite ones lie inside the format then), to four bytes; NaN stays NaN
 __device__ __forceinline__ unsigned lcf_f8_pack4(float a, float b, float c, float d, int fmt)
 {
-    const float nan = __uint_as_float(0x7FC00000u);
-    a = __builtin_fabsf(a) <= 3.402823466e38f ? a : nan;
-    b = __builtin_fabsf(b) <= 3.402823466e38f ? b : nan;
-    c = __builtin_fabsf(c) <= 3.402823466e38f ? c : nan;
-    d = __builtin_fabsf(d) <= 3.402823466e38f ? d : nan;
     int r = 0;
     if (fmt == LCF_E4M3) {
         r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false);

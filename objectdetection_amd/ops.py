@@ -1643,7 +1643,7 @@ def f8_matmul(a, b, scale=None, shift=None, relu=False, out_dtype=torch.float32,
     with _on_device(a.data):
         if out is None:
             out = torch.empty((M, N), dtype=out_dtype, device=dev)
-        nbytes = L.lcf_f8_gemm_workspace_bytes(M, N, K)
+        nbytes = L.lcf_f8_gemm_workspace_bytes(M, N, K, _TYPE_CODE[out.dtype])
         ws = _ws(nbytes, dev) if nbytes else None
         check(L.lcf_f8_gemm(
             _ptr(a.data), a.data.stride(0) if M > 1 else -(-K // 16) * 16, _ptr(a.scale),
@@ -1656,6 +1656,27 @@ def f8_matmul(a, b, scale=None, shift=None, relu=False, out_dtype=torch.float32,
     return out
 
 
+def _f8_product(x, b, shift=None, scale=None, relu=False):
+    """f8_matmul(f8_rows(x), b) of x's own type: one launch where lcf_f8_linear takes the sizes
+    (thin layers over many rows), two elsewhere."""
+    M, K = x.shape
+    N = b.data.shape[0]
+    x, ldx = _rows2d(x.detach(), K)
+    thin = (M >= 4096 and N <= 256 and 0 < K <= (256 if x.dtype == torch.float32 else 512)
+            and K % 8 == 0 and x.data_ptr() % 4 == 0 and ldx * x.element_size() % 4 == 0
+            and ldx <= 1 << 22)
+    if not thin or b.data.dtype != torch.float8_e4m3fn:
+        return f8_matmul(f8_rows(x), b, scale, shift, relu, out_dtype=x.dtype)
+    with _on_device(x):
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        check(_lib.lib().lcf_f8_linear(
+            _ptr(x), ldx, _TYPE_CODE[x.dtype], _ptr(b.data),
+            b.data.stride(0) if N > 1 else -(-K // 16) * 16, _ptr(b.scale), b.scale.stride(0) if
+            b.scale.shape[0] > 1 else 4, int(b.scale.shape[0] != N), M, N, K, _ptr(scale),
+            _ptr(shift), int(bool(relu)), _ptr(out), N, _TYPE_CODE[x.dtype], _stream()))
+    return out
+
+
 class F8LinearFunction(torch.autograd.Function):
     """y = x W^T (+ bias) with x and W rounded to 8-bit form; the three products (y, dx = dy W,
     dW = dy^T x) run on 8-bit operands with fp32 accumulation, each operand's scale blocks lying
@@ -1664,9 +1685,12 @@ class F8LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, turned, x8):
-        y = f8_matmul(f8_rows(x) if x8 is None else x8, f8_weight_image(weight, transpose=turned),
-                      shift=None if bias is None else bias.detach().float().contiguous(),
-                      out_dtype=x.dtype)
+        image = f8_weight_image(weight, transpose=turned)
+        shift = None if bias is None else bias.detach().float().contiguous()
+        if x8 is None:
+            y = _f8_product(x, image, shift)
+        else:
+            y = f8_matmul(x8, image, shift=shift, out_dtype=x.dtype)
         ctx.save_for_backward(x, weight)
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.turned = turned

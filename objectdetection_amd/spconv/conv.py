@@ -172,10 +172,11 @@ class SparseConvolution(SparseModule):
             b = self.bias.detach().float()
             b = b if scale is None else b * scale
             shift = b if shift is None else b + shift
-        return ops.f8_matmul(
-            ops.f8_rows(x) if f8 is None else f8, self._weight_image("f8"),
-            None if scale is None else scale.float().contiguous(),
-            None if shift is None else shift.float().contiguous(), relu, out_dtype=x.dtype)
+        scale = None if scale is None else scale.float().contiguous()
+        shift = None if shift is None else shift.float().contiguous()
+        if f8 is None:
+            return ops._f8_product(x, self._weight_image("f8"), shift, scale, relu)
+        return ops.f8_matmul(f8, self._weight_image("f8"), scale, shift, relu, out_dtype=x.dtype)
 
     def _inference_forward(self, x, rb, scale, shift, relu):
         """No-grad forward: fp32 MFMA, or -- under ``ops.conv_math("bf16x3")`` and for 32 / 64 /

@@ -135,6 +135,29 @@ def test_f8_matmul(cuda, shape):
         _within(got, want, _product_bound(qa, qb, K, want, out), (shape, fa, fb, square))
 
 
+@pytest.mark.parametrize("shape", [(4096, 1, 16), (4100, 64, 64), (5001, 256, 100), (4097, 130, 256), (4200, 200, 512),
+                                   (9000, 65, 129), (4096, 256, 300), (3600, 3500, 330), (3585, 3600, 128)])
+def test_f8_matmul_many_rows(cuda, shape):
+    """Thin layers over many rows, and outputs of many tiles; a linear layer's one launch gives the
+    bits of the two calls."""
+    M, N, K = shape
+    a, b = _rows(4, M, K), _rows(5, N, K, size=K ** -0.5)
+    for fa, fb, square, out in ((E4M3, E4M3, True, torch.float32), (E4M3, E4M3, False, torch.bfloat16),
+                                (E5M2, E5M2, True, torch.float16)):
+        qa = ref.value(*ref.quantise(a, fa))
+        qb = ref.value(*ref.quantise(b, fb, 128 if square else 1), 128 if square else 1)
+        want = qa @ qb.t()
+        xb = ops.f8_weight_image(b.to(cuda), dtype=fb) if square else ops.f8_rows(b.to(cuda), fb)
+        got = ops.f8_matmul(ops.f8_rows(a.to(cuda), fa), xb, out_dtype=out)
+        _within(got, want, _product_bound(qa, qb, K, want, out), (shape, fa, fb, square))
+    w = ops.f8_weight_image(b.to(cuda))
+    shift = torch.randn((N,), generator=_gen(6)).to(cuda)
+    for dtype in DTYPES:
+        x = torch.nn.functional.pad(a.to(dtype).to(cuda), (1, 2))[:, 1:1 + K]
+        want = ops.f8_matmul(ops.f8_rows(x), w, shift=shift, relu=True, out_dtype=dtype)
+        assert torch.equal(ops._f8_product(x, w, shift, relu=True), want)
+
+
 def test_f8_matmul_epilogue_and_out(cuda):
     M, N, K = 70, 150, 200
     a, b = _rows(6, M, K), _rows(7, N, K, size=0.1)
@@ -160,7 +183,7 @@ def test_f8_matmul_epilogue_and_out(cuda):
 def test_f8_matmul_split_sum_is_repeatable_and_joined(cuda):
     M, N, K = 40, 64, 70000
     a, b = _rows(10, M, K), _rows(11, N, K)
-    assert ops._lib.lib().lcf_f8_gemm_workspace_bytes(M, N, K) > 0
+    assert ops._lib.lib().lcf_f8_gemm_workspace_bytes(M, N, K, 0) > 0
     xa, xb = ops.f8_rows(a.to(cuda)), ops.f8_rows(b.to(cuda))
     qa, qb = ref.value(*ref.quantise(a)), ref.value(*ref.quantise(b))
     bias = torch.randn((N,), generator=_gen(12)).to(cuda)
