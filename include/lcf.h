@@ -754,6 +754,8 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  *   columns form (qt / st, NULL = not wanted): the rows form of x^T, [C, R], blocks of 128 along
  *   each column; square != 0: one scale for 128 x 128, and s / st have ceil(R / 128) /
  *   ceil(C / 128) rows.
+ *   sums != NULL: the columns' sums over each 128 rows, [ceil(R / 128), C] fp32, for lcf_sum_parts
+ *   (a bias gradient out of the same reading; q and qt may then both be NULL).
  *   Bytes between the last column and the next multiple of 16, and scale bytes between the last
  *   block and the next multiple of 4, are written as zeros.
  * gemm: out[m][n] = act((sum_k a[m][k] b[n][k]) * scale[n] + shift[n]), a [M, K], b [N, K] in rows
@@ -768,7 +770,9 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  *   order, so results are run-to-run identical). */
 int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtype, int fmt, int square, void *q,
                  long long ldq, unsigned char *s, int lds, void *qt, long long ldqt,
-                 unsigned char *st, int ldst, void *stream);
+                 unsigned char *st, int ldst, float *sums, void *stream);
+/* out [n] of `dtype` = the column sums of parts [count, n], in 64 bits and a fixed order. */
+int lcf_sum_parts(const float *parts, int count, int n, void *out, int dtype, void *stream);
 size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype);
 int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa, int ldsa, int a_fmt,
                 const void *b, long long ldb, const unsigned char *sb, int ldsb, int b_fmt,
@@ -776,8 +780,9 @@ int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa, int ldsa,
                 void *out, long long ldo, int out_dtype, void *ws, size_t ws_bytes, void *stream);
 /* lcf_f8_quant of x (rows form, e4m3) and lcf_f8_gemm against an e4m3 b in ONE launch, the 8-bit rows
  * staying in registers: the same result bit for bit.  For thin layers over many rows with
- * dtype == out_dtype: M >= 4096, N <= 256, K <= 512 (fp32: 256) and a multiple of 8, x and its rows
- * on 4-byte borders; LCF_ERR_UNSUPPORTED otherwise and the caller makes the two calls. */
+ * dtype == out_dtype: M >= 4096, N <= 256 and a multiple of 8 (fp32: 4), K <= 512 (fp32: 256) and a
+ * multiple of 8, x, out and their rows on 4-byte borders; LCF_ERR_UNSUPPORTED otherwise and the
+ * caller makes the two calls. */
 int lcf_f8_linear(const void *x, long long ldx, int dtype, const void *b, long long ldb,
                   const unsigned char *sb, int ldsb, int b_square, int M, int N, int K,
                   const float *scale, const float *shift, int relu, void *out, long long ldo,

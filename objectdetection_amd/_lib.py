@@ -202,7 +202,9 @@ SYMBOLS = {
                                  c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                  c_size_t, c_void_p]),
     "lcf_f8_quant": (c_int, [c_void_p, c_ll, c_int, c_int, c_int, c_int, c_int, c_void_p, c_ll,
-                             c_void_p, c_int, c_void_p, c_ll, c_void_p, c_int, c_void_p]),
+                             c_void_p, c_int, c_void_p, c_ll, c_void_p, c_int, c_void_p,
+                             c_void_p]),
+    "lcf_sum_parts": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
     "lcf_f8_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "lcf_f8_linear": (c_int, [c_void_p, c_ll, c_int, c_void_p, c_ll, c_void_p, c_int, c_int, c_int,
                               c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_ll, c_int,
@@ -273,6 +275,25 @@ def lib():
                 "`make -C objectdetection_amd/csrc`.  There is no CPU fallback.")
         _lib = _Lib(ctypes.CDLL(LIB_PATH))
     return _lib
+
+
+_rows = None
+
+
+def row_ops():
+    """The row operators' host module (csrc/host/row_ops.cpp), bound to the loaded library; raises
+    if it has not been built."""
+    global _rows
+    if _rows is None:
+        L = lib()
+        try:
+            from . import _row_ops
+        except ImportError as e:
+            raise RuntimeError(f"_row_ops.so cannot be loaded ({e}): build it with "
+                               "`make -C objectdetection_amd/csrc`.") from e
+        _row_ops.bind({n: ctypes.cast(getattr(L._cdll, n), c_void_p).value for n in SYMBOLS})
+        _rows = _row_ops
+    return _rows
 
 
 class Context:

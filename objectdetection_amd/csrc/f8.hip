@@ -26,6 +26,7 @@ typedef __bf16 f8_b8 __attribute__((ext_vector_type(8)));
 struct F8Quant {
     const void *x;
     unsigned char *q, *s, *qt, *st;
+    float *sums;
     long long ldx, ldq, ldqt;
     int R, C, lds, ldst, fmt, square;
 };
@@ -50,8 +51,12 @@ template <typename T, int LPB> __global__ void __launch_bounds__(256) f8_rows_ke
         for (int i = 0; i < 8; ++i) v[i] = 0.f;
         if (live && col < p.C) lcf_ld8_tail((const T *)p.x + row * p.ldx, col, p.C, v);
         float top = lcf_f8_top<8>(v);
+        if constexpr (LPB == 16) {
+            top = lcf_max16(top);
+        } else {
 #pragma unroll
-        for (int d = LPB / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            for (int d = LPB / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        }
         const int e = lcf_f8_exponent(top, p.fmt);
         const float s = lcf_exp2i(-e);
         if (live && col < room) {
@@ -70,66 +75,92 @@ template <typename T, int LPB> __global__ void __launch_bounds__(256) f8_rows_ke
 }
 
 // Any of the forms from one reading: a workgroup takes 128 x 128 elements.  Thread (rl, cl) holds
-// rows rl + 16 i (i < 8) and columns 8 cl .. 8 cl + 7; a row's magnitudes meet over the 16 lanes of
-// equal rl, a column's over the thread's own rows, the wave's four row lanes and, through LDS, the
-// four waves.  The transposed bytes are turned in LDS and leave as 16-byte pieces of whole rows.
-#define F8_TP 144 // bytes of a transposed row in LDS: 128 and a pad of 16 (other banks for the next)
+// rows 8 rl .. 8 rl + 7 and columns 8 cl .. 8 cl + 7: a row's magnitudes meet over the 16 lanes of
+// equal rl (rotations on the vector unit), a column's over the thread's own rows, the wave's four row
+// lanes and, through LDS, the four waves.  Eight bytes of a transposed row are one thread's own;
+// they are turned in LDS, four at a time, and leave as 16-byte pieces of whole rows.  (A thread with
+// every 16th row wrote single bytes to two of the 64 banks: 84 us for 136000 x 256 bf16, both forms.)
+#define F8_TP 132 // bytes of a transposed row in LDS: eight rows further on start 32 bytes further on
 template <typename T> __global__ void __launch_bounds__(256) f8_tile_kernel(F8Quant p)
 {
     __shared__ float colmax[4][128];
-    __shared__ __align__(16) unsigned char turn[128 * F8_TP];
+    __shared__ unsigned turn[128 * F8_TP / 4];
     const int tid = threadIdx.x, cl = tid & 15, rl = tid >> 4, wave = tid >> 6;
     const int r0 = blockIdx.y * 128, c0 = blockIdx.x * 128;
     const int col = c0 + cl * 8;
-    float v[8][8];
+    float v[8][8], rm[8], cm[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int row = r0 + rl + i * 16;
+        const int row = r0 + rl * 8 + i;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
         if (row < p.R && col < p.C) lcf_ld8_tail((const T *)p.x + row * p.ldx, col, p.C, v[i]);
     }
-    float cm[8];
-    lcf_f8_top<64>(&v[0][0]); // infinities out first
+    if (p.sums) { // the columns' sums over these 128 rows
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        cm[j] = 0.f;
+        for (int j = 0; j < 8; ++j) {
+            float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cm[j] = fmaxf(cm[j], __builtin_fabsf(v[i][j]));
-        cm[j] = fmaxf(cm[j], __shfl_xor(cm[j], 16, 64));
-        cm[j] = fmaxf(cm[j], __shfl_xor(cm[j], 32, 64));
+            for (int i = 0; i < 8; ++i) s += v[i][j];
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            if ((tid & 63) < 16) colmax[wave][cl * 8 + j] = s;
+        }
+        __syncthreads();
+        if (tid < 128 && c0 + tid < p.C)
+            p.sums[(long long)blockIdx.y * p.C + c0 + tid] =
+                (colmax[0][tid] + colmax[1][tid]) + (colmax[2][tid] + colmax[3][tid]);
+        __syncthreads();
     }
-    if ((tid & 63) < 16) {
+    float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) colmax[wave][cl * 8 + j] = cm[j];
+    for (int i = 0; i < 8; ++i) {
+        rm[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rm[i] = fmaxf(rm[i], __builtin_fabsf(v[i][j]));
+        top = fmaxf(top, rm[i]);
     }
-    __syncthreads();
-    float all = 0.f;
+    if (__builtin_expect(__any(top > 3.402823466e38f), 0)) { // infinities become NaN
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+        for (int i = 0; i < 8; ++i) {
+            rm[i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) cm[j] = fmaxf(cm[j], colmax[w][cl * 8 + j]);
-        all = fmaxf(all, cm[j]);
+            for (int j = 0; j < 8; ++j) {
+                if (__builtin_fabsf(v[i][j]) > 3.402823466e38f) v[i][j] = __uint_as_float(0x7FC00000u);
+                rm[i] = fmaxf(rm[i], __builtin_fabsf(v[i][j]));
+            }
+        }
     }
-    if (p.square) {
+    int esq = 0;
+    if (p.qt || p.square) {
 #pragma unroll
-        for (int d = 8; d >= 1; d >>= 1) all = fmaxf(all, __shfl_xor(all, d, 64));
+        for (int j = 0; j < 8; ++j) {
+            cm[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) cm[j] = fmaxf(cm[j], __builtin_fabsf(v[i][j]));
+            cm[j] = fmaxf(cm[j], __shfl_xor(cm[j], 16, 64));
+            cm[j] = fmaxf(cm[j], __shfl_xor(cm[j], 32, 64));
+        }
+        if ((tid & 63) < 16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) colmax[wave][cl * 8 + j] = cm[j];
+        }
+        __syncthreads();
+        float all = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) cm[j] = fmaxf(cm[j], colmax[w][cl * 8 + j]);
+            all = fmaxf(all, cm[j]);
+        }
+        esq = lcf_f8_exponent(lcf_max16(all), p.fmt);
     }
-    const int esq = lcf_f8_exponent(all, p.fmt);
     if (p.q) {
         const int room = (p.C + 15) & ~15;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int row = r0 + rl + i * 16;
-            int e = esq;
-            if (!p.square) {
-                float top = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, __builtin_fabsf(v[i][j]));
-#pragma unroll
-                for (int d = 8; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-                e = lcf_f8_exponent(top, p.fmt);
-            }
+            const int row = r0 + rl * 8 + i;
+            const int e = p.square ? esq : lcf_f8_exponent(lcf_max16(rm[i]), p.fmt);
             const float s = lcf_exp2i(-e);
             if (row < p.R && col < room) {
                 lcf_u2u o;
@@ -146,45 +177,36 @@ template <typename T> __global__ void __launch_bounds__(256) f8_tile_kernel(F8Qu
         }
     }
     if (p.qt) {
-        int e[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            e[j] = p.square ? esq : lcf_f8_exponent(cm[j], p.fmt);
-            const float s = lcf_exp2i(-e[j]);
-            const unsigned a = lcf_f8_pack4(v[0][j] * s, v[1][j] * s, v[2][j] * s, v[3][j] * s, p.fmt);
-            const unsigned b = lcf_f8_pack4(v[4][j] * s, v[5][j] * s, v[6][j] * s, v[7][j] * s, p.fmt);
-            unsigned char *t = turn + (cl * 8 + j) * F8_TP + rl;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                t[i * 16] = (unsigned char)(a >> (8 * i));
-                t[i * 16 + 64] = (unsigned char)(b >> (8 * i));
-            }
-        }
-        if (rl == 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (p.square ? (cl == 0 && j == 0) : col + j < p.C) {
-                    unsigned char *sr = p.st + (long long)(p.square ? blockIdx.x : col + j) * p.ldst;
-                    sr[blockIdx.y] = (unsigned char)(e[j] + 127);
-                    if (blockIdx.y == gridDim.y - 1)
-                        for (int k = gridDim.y; k & 3; ++k) sr[k] = 0;
-                }
+            const int e = p.square ? esq : lcf_f8_exponent(cm[j], p.fmt);
+            const float s = lcf_exp2i(-e);
+            unsigned *t = turn + (cl * 8 + j) * (F8_TP / 4) + rl * 2;
+            t[0] = lcf_f8_pack4(v[0][j] * s, v[1][j] * s, v[2][j] * s, v[3][j] * s, p.fmt);
+            t[1] = lcf_f8_pack4(v[4][j] * s, v[5][j] * s, v[6][j] * s, v[7][j] * s, p.fmt);
+            if (rl == 0 && (p.square ? (cl == 0 && j == 0) : col + j < p.C)) {
+                unsigned char *sr = p.st + (long long)(p.square ? blockIdx.x : col + j) * p.ldst;
+                sr[blockIdx.y] = (unsigned char)(e + 127);
+                if (blockIdx.y == gridDim.y - 1)
+                    for (int k = gridDim.y; k & 3; ++k) sr[k] = 0;
             }
         }
         __syncthreads();
         const int room = (p.R + 15) & ~15;
-        for (int k = tid; k < 128 * 8; k += 256) {
-            const int c = k >> 3, part = (k & 7) * 16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = (tid >> 3) + k * 32, part = (tid & 7) * 16;
+            const unsigned *t = turn + c * (F8_TP / 4) + part / 4;
             if (c0 + c < p.C && r0 + part < room)
                 *reinterpret_cast<uint4 *>(p.qt + (long long)(c0 + c) * p.ldqt + r0 + part) =
-                    *reinterpret_cast<const uint4 *>(turn + c * F8_TP + part);
+                    make_uint4(t[0], t[1], t[2], t[3]);
         }
     }
 }
 
 template <typename T> static void f8_quant_launch(const F8Quant &p, hipStream_t st)
 {
-    if (p.q && !p.qt && !p.square) {
+    if (p.q && !p.qt && !p.square && !p.sums) {
         const long long blocks = (long long)p.R * ((p.C + 127) / 128);
         auto grid = [&](int lpb) {
             const long long g = (blocks * lpb + 255) / 256;
@@ -207,16 +229,16 @@ static bool f8_form_ok(const void *q, long long ld, const unsigned char *s, int 
 
 extern "C" int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtype, int fmt, int square, void *q,
                             long long ldq, unsigned char *s, int lds, void *qt, long long ldqt, unsigned char *st,
-                            int ldst, void *stream)
+                            int ldst, float *sums, void *stream)
 {
     if (R < 0 || C < 0 || !lcf_is_type(dtype) || (fmt != LCF_E4M3 && fmt != LCF_E5M2)) return LCF_ERR_ARG;
     if (R == 0 || C == 0) return LCF_OK;
-    if (!x || ldx < C || (!q && !qt)) return LCF_ERR_ARG;
+    if (!x || ldx < C || (!q && !qt && !sums)) return LCF_ERR_ARG;
     if (q && !f8_form_ok(q, ldq, s, lds, C)) return LCF_ERR_ARG;
     if (qt && !f8_form_ok(qt, ldqt, st, ldst, R)) return LCF_ERR_ARG;
     // the grid's second dimension counts 128-row tiles
-    if ((qt || square) && (R + 127) / 128 > 65535) return LCF_ERR_UNSUPPORTED;
-    F8Quant p{x, (unsigned char *)q, s, (unsigned char *)qt, st, ldx, ldq, ldqt, R, C, lds, ldst, fmt, square};
+    if ((qt || square || sums) && (R + 127) / 128 > 65535) return LCF_ERR_UNSUPPORTED;
+    F8Quant p{x, (unsigned char *)q, s, (unsigned char *)qt, st, sums, ldx, ldq, ldqt, R, C, lds, ldst, fmt, square};
     if (dtype == LCF_F32) f8_quant_launch<float>(p, (hipStream_t)stream);
     else if (dtype == LCF_BF16) f8_quant_launch<lcf_b>(p, (hipStream_t)stream);
     else f8_quant_launch<lcf_h>(p, (hipStream_t)stream);
@@ -272,14 +294,13 @@ template <int W> __device__ __forceinline__ void f8_store(const F8Gemm &p, long 
     else put((lcf_h *)p.out + m * p.ldo + n);
 }
 
-// bytes [col, col + 16) of a row of K: those behind the row's end become zeros
+// bytes [col, col + 16) of a row of K: those behind the row's end become zeros (no branches: masks)
 __device__ __forceinline__ void f8_cut(int *w, int col, int K)
 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int left = K - (col + 4 * i);
-        if (left <= 0) w[i] = 0;
-        else if (left < 4) w[i] &= (1 << (8 * left)) - 1;
+        const int left = min(max(K - (col + 4 * i), 0), 4);
+        w[i] &= left == 4 ? -1 : (1 << (8 * left)) - 1;
     }
 }
 
@@ -565,9 +586,11 @@ __global__ void __launch_bounds__(WM *WN * 64) f8_gemm_kernel(F8Gemm p)
 // its 64 columns of b (all of K: 32 KS registers, 64 KS widened) and walks down the rows, 16 at a
 // time, straight from memory to the matrix core and back: nothing goes through LDS and nothing
 // waits for another wave.  The waves of a workgroup that share rows read them through the same L1.
-// The next 16 rows are asked for before this one's are used.  Their loads stand behind no branch
-// (a load behind one would make every later wait assume the worst): what lies past the last row or
-// past K is an offset beyond the buffer's end, which brings zeros and touches no memory.
+// The next 16 rows are asked for before this one's are used, and no load or store of the loop stands
+// behind a branch: memory operations are counted in order, and one that may not have happened makes
+// the wait for the rows a wait for the stores in front of them as well (5 us a turn).  What lies
+// past the last row, past K or past N is an offset beyond its buffer's end instead: such a load
+// brings zeros and such a store is dropped, neither touches memory.  Scale and shift wait in LDS.
 // T: the rows are fp32 / bf16 / fp16 and brought into 8-bit form in registers on the way (bit for
 // bit what f8_rows_kernel stores: a row's 128 columns are in the four lanes of equal r16), which
 // saves writing and reading them; T = unsigned char: they are in that form already.
@@ -578,39 +601,15 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const int n0 = (wave & ((1 << wn_shift) - 1)) * 64;
+    __shared__ __align__(16) float affine[2][256];
+    {
+        const int n = threadIdx.x;
+        affine[0][n] = p.scale && n < p.N ? p.scale[n] : 1.f;
+        affine[1][n] = p.shift && n < p.N ? p.shift[n] : 0.f;
+    }
+    __syncthreads();
     if (n0 >= p.N) return;
     const int rows = 16 << (2 - wn_shift), wm = (wave >> wn_shift) * 16; // rows a workgroup takes at a time
-
-    f8_v8 fb[KS][4];
-    unsigned xb[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int n = min(n0 + f8_column<WIDE>(t, r16), p.N - 1);
-        xb[t] = *(const unsigned *)(p.sb + (long long)(n >> p.b_shift) * p.ldsb);
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int col = k * 128 + g * 16 + h * 64;
-                f8_v4 v = (f8_v4){0, 0, 0, 0};
-                if (col < p.K) v = *reinterpret_cast<const f8_v4 *>(p.b + (long long)n * p.ldb + col);
-                int w[4] = {v[0], v[1], v[2], v[3]};
-                f8_cut(w, col, p.K);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) fb[k][t][h * 4 + i] = w[i];
-            }
-    }
-    f8_b8 wb[WIDE ? KS : 1][4][4];
-    if constexpr (WIDE) {
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    wb[k][t][q] = f8_to_bf16<FB>(fb[k][t][2 * q], fb[k][t][2 * q + 1],
-                                                 lcf_exp2i((int)((xb[t] >> (8 * k)) & 255) - 127));
-    }
 
     // piece i of step k holds elements col .. col + 16 / E of the row: the lane's 16 columns from
     // 16 g on, then the 16 from 64 + 16 g on
@@ -641,6 +640,63 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
             x.s = *(const unsigned *)(p.sa + m * p.ldsa);
         }
     };
+    const long long stride = (long long)gridDim.x * rows;
+    long long m0 = (long long)blockIdx.x * rows + wm;
+    // two sets of registers used in turn: copying one to the other would wait for it
+    Rows x, y;
+    ask(m0, x);
+
+    f8_v8 fb[KS][4];
+    unsigned xb[4];
+    {
+        // all of b at once, then the cuts: one round trip
+        const __amdgpu_buffer_rsrc_t buf = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<unsigned char *>(p.b + (long long)n0 * p.ldb), 0,
+            (min(64, p.N - n0) - 1) * (int)p.ldb + ((p.K + 15) & ~15), 0x00020000);
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int n = min(f8_column<WIDE>(t, r16), p.N - 1 - n0);
+            xb[t] = *(const unsigned *)(p.sb + (long long)((n0 + n) >> p.b_shift) * p.ldsb);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = k * 128 + g * 16 + h * 64;
+                    const u4 v = __builtin_amdgcn_raw_buffer_load_b128(
+                        buf, col < p.K ? n * (int)p.ldb + col : (int)0x80000000, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) fb[k][t][h * 4 + i] = (int)v[i];
+                }
+        }
+        if (p.K & 15) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        int w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = fb[k][t][h * 4 + i];
+                        f8_cut(w, k * 128 + g * 16 + h * 64, p.K);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) fb[k][t][h * 4 + i] = w[i];
+                    }
+        }
+    }
+    f8_b8 wb[WIDE ? KS : 1][4][4];
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    wb[k][t][q] = f8_to_bf16<FB>(fb[k][t][2 * q], fb[k][t][2 * q + 1],
+                                                 lcf_exp2i((int)((xb[t] >> (8 * k)) & 255) - 127));
+    }
+
     auto use = [&](long long m0, const Rows &x) {
         int fa[KS][8];
         unsigned xa = 0;
@@ -702,16 +758,59 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
             }
         }
         f8_pin(acc);
-        if (m0 + r16 < p.M) f8_put<WIDE>(p, nullptr, m0 + r16, n0, g, acc);
+        constexpr int W = WIDE ? 4 : 8, EO = WIDE ? 4 : 2;
+        const int left = p.M - m0 < 16 ? (int)(p.M - m0) : 16;
+        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+            (char *)p.out + m0 * p.ldo * EO, 0, ((left - 1) * (int)p.ldo + p.N) * EO, 0x00020000);
+#pragma unroll
+        for (int q = 0; q < 16 / W; ++q) {
+            const int n = n0 + (WIDE ? 16 * q + 4 * g : 32 * q + 8 * g);
+            float v[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = acc[WIDE ? q : 2 * q + (i >> 2)][i & 3];
+            if (p.scale) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] *= affine[0][n + i];
+            }
+            if (p.shift) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] += affine[1][n + i];
+            }
+            if (p.relu) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] = v[i] < 0.f ? 0.f : v[i]; // NaN stays
+            }
+            typedef unsigned u4 __attribute__((ext_vector_type(4)));
+            u4 o;
+            if constexpr (WIDE) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = __float_as_uint(v[i]);
+            } else if (p.code == LCF_BF16) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[i] = __builtin_bit_cast(unsigned short, lcf_from_f32<lcf_b>(v[2 * i])) |
+                           (unsigned)__builtin_bit_cast(unsigned short, lcf_from_f32<lcf_b>(v[2 * i + 1])) << 16;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[i] = __builtin_bit_cast(unsigned short, lcf_from_f32<lcf_h>(v[2 * i])) |
+                           (unsigned)__builtin_bit_cast(unsigned short, lcf_from_f32<lcf_h>(v[2 * i + 1])) << 16;
+            }
+            // N is a multiple of W: a piece is inside or outside as a whole
+            const int at = n < p.N && r16 < left ? (r16 * (int)p.ldo + n) * EO : (int)0x80000000;
+            __builtin_amdgcn_raw_buffer_store_b128(o, to, at, 0, 0);
+        }
     };
-    const long long stride = (long long)gridDim.x * rows;
-    long long m0 = (long long)blockIdx.x * rows + wm;
-    Rows x, next;
-    ask(m0, x);
-    for (; m0 < p.M; m0 += stride) {
-        ask(m0 + stride, next);
+    // everything asked for so far is here: the loop's waits then count its own operations only
+    __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0)
+    while (m0 < p.M) {
+        ask(m0 + stride, y);
         use(m0, x);
-        x = next;
+        m0 += stride;
+        if (m0 >= p.M) break;
+        ask(m0 + stride, x);
+        use(m0, y);
+        m0 += stride;
     }
 }
 
@@ -792,10 +891,17 @@ extern "C" size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype
     return q.splits > 1 ? (size_t)q.splits * M * N * sizeof(float) : 0;
 }
 
-// whether f8_stream_kernel takes a product: b in registers, and rows enough for every wave
+// whether f8_stream_kernel takes a product: b in registers, rows enough for every wave, and whole
+// 16-byte pieces of an output row
 static bool f8_is_thin(int M, int N, int K, bool wide)
 {
-    return K > 0 && K <= (wide ? 256 : 512) && N <= 256 && M >= 4096;
+    return K > 0 && K <= (wide ? 256 : 512) && N <= 256 && N % (wide ? 4 : 8) == 0 && M >= 4096;
+}
+// (buffer stores want four-byte addresses; an output that has none takes the tiles, which for these
+// sizes are never split and need no workspace either)
+static bool f8_out_ok(const void *out, long long ldo, int code)
+{
+    return !((uintptr_t)out & 3) && !(ldo * lcf_type_size(code) & 3) && ldo <= (1 << 22);
 }
 
 template <int FA, int FB, bool WIDE, typename T> static int f8_stream_launch(const F8Gemm &p, hipStream_t st)
@@ -814,7 +920,7 @@ template <int FA, int FB, bool WIDE, typename T> static int f8_stream_launch(con
 
 template <int FA, int FB, bool WIDE> static int f8_gemm_launch2(const F8Gemm &p, const F8Plan &q, hipStream_t st)
 {
-    if (q.thin) return f8_stream_launch<FA, FB, WIDE, unsigned char>(p, st);
+    if (q.thin && f8_out_ok(p.out, p.ldo, p.code)) return f8_stream_launch<FA, FB, WIDE, unsigned char>(p, st);
     const unsigned grid = (unsigned)(((long long)q.tiles_m * q.tiles_n * q.splits + 7) / 8 * 8);
     // more LDS than a launch may take unasked
     if (q.big) {
@@ -847,7 +953,8 @@ extern "C" int lcf_f8_linear(const void *x, long long ldx, int dtype, const void
     if (K > 0 && (!x || ldx < K || !f8_form_ok(b, ldb, sb, ldsb, K))) return LCF_ERR_ARG;
     // rows are read 16 bytes at a time, by buffer loads that want four-byte addresses
     if (!f8_is_thin(M, N, K, out_dtype == LCF_F32) || dtype != out_dtype || (K & 7) || ((uintptr_t)x & 3) ||
-        (ldx * lcf_type_size(dtype) & 3) || ldx > (1 << 22) || ldb > (1 << 22))
+        (ldx * lcf_type_size(dtype) & 3) || ldx > (1 << 22) || ldb > (1 << 22) ||
+        !f8_out_ok(out, ldo, out_dtype))
         return LCF_ERR_UNSUPPORTED;
     F8Gemm p{};
     p.a = (const unsigned char *)x;

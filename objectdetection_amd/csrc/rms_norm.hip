@@ -105,8 +105,12 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) rn_fwd_kernel(RnFwd p)
                         if (col + i >= p.width) h[c][i] = 0.f;
                 }
                 float top = lcf_f8_top<8>(h[c]);
+                if constexpr (LPR >= 16) {
+                    top = lcf_max16(top);
+                } else {
 #pragma unroll
-                for (int d = (LPR < 16 ? LPR : 16) / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+                    for (int d = LPR / 2; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+                }
                 const int e = lcf_f8_exponent(top, p.fmt);
                 const float s = lcf_exp2i(-e);
                 if (live && col < ((p.width + 15) & ~15)) {
@@ -357,5 +361,15 @@ extern "C" int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, lo
         rn_dweight_kernel<<<(width + 15) / 16, 1024, 0, st>>>((const float *)ws, grid, width, dweight, weight_dtype);
         LCF_CHECK_LAUNCH();
     }
+    return LCF_OK;
+}
+
+extern "C" int lcf_sum_parts(const float *parts, int count, int n, void *out, int dtype, void *stream)
+{
+    if (count < 0 || n < 0 || !lcf_is_type(dtype)) return LCF_ERR_ARG;
+    if (n == 0) return LCF_OK;
+    if ((count > 0 && !parts) || !out) return LCF_ERR_ARG;
+    rn_dweight_kernel<<<(n + 15) / 16, 1024, 0, (hipStream_t)stream>>>(parts, count, n, out, dtype);
+    LCF_CHECK_LAUNCH();
     return LCF_OK;
 }

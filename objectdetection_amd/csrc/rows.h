@@ -145,3 +145,17 @@ __device__ __forceinline__ unsigned lcf_f8_pack4(float a, float b, float c, floa
     }
     return (unsigned)r;
 }
+
+// the largest of the 16 lanes of a row of lanes, in all of them: four rotations on the vector unit
+// (a shuffle would go through LDS)
+__device__ __forceinline__ float lcf_max16(float v)
+{
+#define LCF_ROR(n) \
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + n, 0xF, 0xF, false)))
+    LCF_ROR(8);
+    LCF_ROR(4);
+    LCF_ROR(2);
+    LCF_ROR(1);
+#undef LCF_ROR
+    return v;
+}

@@ -4,7 +4,6 @@ PyTorch is plumbing here: it owns device memory and streams; every computation i
 in liblcf.so enqueued on torch's current stream.  Nothing in this module has a CPU fallback:
 tensors must live on the GPU, and the library must have been built.
 """
-from array import array
 from collections import namedtuple
 
 import torch
@@ -1248,77 +1247,34 @@ _F8_CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}  # LCF_E4M3, LCF_E5M2
 _NORM_CODE = {1: 1, 1.0: 1, 2: 2, 2.0: 2, float("inf"): 0}
 
 
-class _on_device:
-    """The device of tensor ``t`` made current for a call (kernels are launched on the current
-    device's stream); nothing to do in the usual case that it is already."""
-
-    def __init__(self, t):
-        self.index = t.get_device()
-        self.prev = None
-
-    def __enter__(self):
-        cur = torch.cuda.current_device()
-        if cur != self.index:
-            self.prev = cur
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            torch.cuda.set_device(self.prev)
+def _row_call(fn, t, *args):
+    """fn(*args, stream) of the row operators' host module on the device of ``t`` (kernels go to that
+    device's current stream)."""
+    index = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if index < 0 or index == torch.cuda.current_device():
+        # a tensor off the GPU is refused by fn itself, before any launch
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index) if index >= 0 else 0)
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _dense_gradient(t):
-    """True if t's elements fill one run of memory (any order of its dimensions)."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if st != want:
-            return t.numel() == 0
-        want *= n
-    return True
-
-
-def _norm_args(tensors, norm_type):
-    tensors = list(tensors)
-    if norm_type not in _NORM_CODE:
-        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
-    if not tensors:
-        return tensors, None, None, None
-    where = {t.get_device() for t in tensors}
-    if -1 in where:
-        _need_cuda(*tensors)
-    if len(where) != 1:
-        raise RuntimeError("the tensors of one norm must be on one device")
+def _f8_code(dtype):
     try:
-        codes = [_TYPE_CODE[t.dtype] for t in tensors]
+        return _F8_CODE[dtype]
     except KeyError:
-        raise TypeError("gradients must be float32, bfloat16 or float16") from None
-    for t in tensors:
-        if not t.is_contiguous() and not _dense_gradient(t):
-            raise ValueError("gradients must be dense in memory (got strides "
-                             f"{tuple(t.stride())} for {tuple(t.shape)}): pass .contiguous()")
-    return tensors, [t.data_ptr() for t in tensors], [t.numel() for t in tensors], codes
+        raise TypeError(f"8-bit rows are float8_e4m3fn or float8_e5m2, got {dtype}") from None
 
 
 def grad_norm(tensors, norm_type=2.0):
     """The norm of all elements of ``tensors`` (float32 / bfloat16 / float16, dense, one device)
     as one vector: norm_type 1, 2 or inf -> 0-d float32 tensor.  Summed in 64 bits in a fixed
     order; no synchronisation.  include/lcf.h: lcf_grad_norm."""
-    tensors, ptrs, sizes, codes = _norm_args(tensors, norm_type)
+    if norm_type not in _NORM_CODE:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
+    tensors = list(tensors)
     if not tensors:
         return torch.zeros(())
-    table = array("q", [0]) * (4 * len(tensors))
-    table[0::4], table[2::4], table[3::4] = (array("q", ptrs), array("q", sizes),
-                                             array("q", codes))
-    L = _lib.lib()
-    with _on_device(tensors[0]):
-        dev = tensors[0].device
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = _ws(L.lcf_grad_norm_workspace_bytes(len(tensors)), dev)
-        check(L.lcf_grad_norm(table.buffer_info()[0], len(tensors), _NORM_CODE[norm_type],
-                              _ptr(norm), _ptr(ws), ws.numel(), _stream()))
-    return norm
+    return _row_call(_lib.row_ops().clip, tensors[0], tensors, None, _NORM_CODE[norm_type], None)
 
 
 def clip_norm_(tensors, max_norm, norm_type=2.0, out=None):
@@ -1331,40 +1287,17 @@ def clip_norm_(tensors, max_norm, norm_type=2.0, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    tensors, ptrs, sizes, codes = _norm_args(tensors, norm_type)
-    if out is None:
-        optrs, ocodes = ptrs, codes
-    elif isinstance(out, torch.Tensor):
-        if not out.is_contiguous() or out.dtype not in _TYPE_CODE or (tensors and (
-                out.get_device() != tensors[0].get_device() or out.numel() != sum(sizes))):
-            raise ValueError("out must be a contiguous float tensor on the gradients' device with "
-                             "as many elements as they have together")
-        code, step, at = _TYPE_CODE[out.dtype], out.element_size(), out.data_ptr()
-        optrs = []
-        for n in sizes or ():
-            optrs.append(at)
-            at += n * step
-        ocodes = [code] * len(tensors)
-    else:
-        out, optrs, osizes, ocodes = _norm_args(out, norm_type)
-        if len(out) != len(tensors) or osizes != sizes or (
-                out and out[0].get_device() != tensors[0].get_device()) or any(
-                o.stride() != t.stride() for o, t in zip(out, tensors) if o.numel() > 1):
-            raise ValueError("out must be tensors of the gradients' sizes, strides and device")
+    if norm_type not in _NORM_CODE:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type!r}")
+    tensors = list(tensors)
+    if out is not None and not isinstance(out, torch.Tensor):
+        out = list(out)
     if not tensors:
+        if out is not None and sum(o.numel() for o in ([out] if isinstance(out, torch.Tensor)
+                                                       else out)):
+            raise ValueError("out must have a tensor for each gradient")
         return torch.zeros(())
-    table = array("q", [0]) * (4 * len(tensors))
-    table[0::4], table[1::4], table[2::4] = (array("q", ptrs), array("q", optrs),
-                                             array("q", sizes))
-    table[3::4] = array("q", [c | o << 32 for c, o in zip(codes, ocodes)])
-    L = _lib.lib()
-    with _on_device(tensors[0]):
-        dev = tensors[0].device
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = _ws(L.lcf_grad_norm_workspace_bytes(len(tensors)), dev)
-        check(L.lcf_grad_clip(table.buffer_info()[0], len(tensors), _NORM_CODE[norm_type],
-                              max_norm, _ptr(norm), _ptr(ws), ws.numel(), _stream()))
-    return norm
+    return _row_call(_lib.row_ops().clip, tensors[0], tensors, out, _NORM_CODE[norm_type], max_norm)
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
@@ -1372,73 +1305,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     clips every ``.grad`` in place and returns the total norm."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    return clip_norm_([p.grad.detach() for p in parameters if p.grad is not None], max_norm,
-                      norm_type)
+    return clip_norm_([p.grad for p in parameters if p.grad is not None], max_norm, norm_type)
 
 
 # ------------------------------------------------------------------ RMS norm of rows
-
-RMS_NORM_MAX_WIDTH = 16384
-
-
-def _rows2d(x, width):
-    """x [..., width] as (2-D view or copy with unit stride in a row, elements between rows)."""
-    if x.dim() != 2:
-        x = x.reshape(-1, width)
-    if x.shape[0] > 1 and (x.stride(0) < width or (x.stride(1) != 1 and width > 1)):
-        x = x.contiguous()
-    elif x.shape[0] <= 1 and width > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    return x, (x.stride(0) if x.shape[0] > 1 else width)
-
-
-def _check_rms(x, weight, residual, eps):
-    _need_cuda(x, weight, residual)
-    if x.dtype not in _TYPE_CODE or x.dim() < 1:
-        raise TypeError(f"rms_norm: rows must be float32, bfloat16 or float16, got {x.dtype}")
-    width = x.shape[-1]
-    if not 1 <= width <= RMS_NORM_MAX_WIDTH:
-        raise ValueError(f"rms_norm: 1 to {RMS_NORM_MAX_WIDTH} columns, got {width}")
-    if weight is not None and (weight.dtype not in _TYPE_CODE or tuple(weight.shape) != (width,)):
-        raise ValueError(f"rms_norm: weight must be a float tensor of {width} elements")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("rms_norm: residual must have x's shape and type")
-    for t in (weight, residual):
-        if t is not None and t.get_device() != x.get_device():
-            raise RuntimeError("rms_norm: all tensors must be on one device")
-    if not float(eps) >= 0.0:
-        raise ValueError(f"rms_norm: eps must not be negative, got {eps}")
-
-
-def _rms_fwd(x, weight, eps, residual, want_y, want_inv, f8):
-    """-> (y, h, inv, F8Rows); y / inv / F8Rows None where not wanted, h = x without a residual."""
-    width = x.shape[-1]
-    x2, ldx = _rows2d(x, width)
-    rows = x2.shape[0]
-    if rows >= 1 << 31:
-        raise ValueError("rms_norm: fewer than 2^31 rows")
-    L = _lib.lib()
-    with _on_device(x):
-        dev = x.device
-        r2, ldr, h = None, 0, x
-        if residual is not None:
-            r2, ldr = _rows2d(residual, width)
-            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_y else None
-        inv = torch.empty((rows,), dtype=torch.float32, device=dev) if want_inv else None
-        q8, ldq, lds = None, 0, 0
-        if f8 is not None:
-            q8 = _f8_empty(rows, width, rows, f8, dev)
-            ldq, lds = q8.data.stride(0), q8.scale.stride(0)
-        w = None if weight is None else weight.contiguous()
-        check(L.lcf_rms_norm_fwd(
-            _ptr(x2), ldx, _ptr(r2), ldr, rows, width, _TYPE_CODE[x.dtype], _ptr(w),
-            0 if w is None else _TYPE_CODE[w.dtype], float(eps), _ptr(y),
-            _ptr(h) if residual is not None else None, _ptr(inv),
-            None if q8 is None else _ptr(q8.data), ldq, None if q8 is None else _ptr(q8.scale), lds,
-            0 if f8 is None else _F8_CODE[f8], _stream()))
-    return y, h, inv, q8
-
 
 class RMSNormFunction(torch.autograd.Function):
     """(y, h) = RMS norm of x (+ residual); backward by lcf_rms_norm_bwd from h and the rows'
@@ -1446,38 +1316,21 @@ class RMSNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, eps, residual):
-        y, h, inv, _ = _rms_fwd(x, weight, eps, residual, True, True, None)
-        ctx.save_for_backward(h, weight, inv)
-        ctx.two = residual is not None
+        y, h, inv, _, _ = _row_call(_lib.row_ops().rms_fwd, x, x, weight, eps, residual, True, True,
+                                    -1)
+        ctx.save_for_backward(x if h is None else h, weight, inv)
+        ctx.two = h is not None
         ctx.set_materialize_grads(False)
-        if ctx.two:
-            return y, h
-        return y
+        return (y, h) if ctx.two else y
 
     @staticmethod
     def backward(ctx, dy, dh=None):
         h, weight, inv = ctx.saved_tensors
-        if dy is None and dh is None:
-            return None, None, None, None
-        width = h.shape[-1]
         need_w = weight is not None and ctx.needs_input_grad[1]
         if dy is None:  # the norm's output was not used: the sum's gradient passes through
-            dw = torch.zeros_like(weight) if need_w else None
+            dw = torch.zeros_like(weight) if need_w and dh is not None else None
             return dh, dw, None, dh if ctx.two else None
-        h2, ldh = _rows2d(h, width)
-        dy2, lddy = _rows2d(dy.to(h.dtype), width)
-        rows = h2.shape[0]
-        L = _lib.lib()
-        with _on_device(h):
-            dh2, lddh = (None, 0) if dh is None else _rows2d(dh.to(h.dtype), width)
-            dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-            dw = torch.empty((width,), dtype=weight.dtype, device=h.device) if need_w else None
-            ws = _ws(L.lcf_rms_norm_workspace_bytes(rows, width), h.device) if need_w else None
-            w = None if weight is None else weight.contiguous()
-            check(L.lcf_rms_norm_bwd(
-                _ptr(h2), ldh, _ptr(dy2), lddy, _ptr(dh2), lddh, rows, width,
-                _TYPE_CODE[h.dtype], _ptr(w), 0 if w is None else _TYPE_CODE[w.dtype], _ptr(inv),
-                _ptr(dx), _ptr(dw), _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
+        dx, dw = _row_call(_lib.row_ops().rms_bwd, h, h, weight, inv, dy, dh, need_w)
         return dx, dw, None, dx if ctx.two else None
 
 
@@ -1487,11 +1340,10 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None):
     h = x + residual rounded to the rows' type, and (y, h) is returned; without it h = x and y is.
     Sums are held in 32 bits.  Differentiable in x, weight and residual.  include/lcf.h:
     lcf_rms_norm_fwd / _bwd."""
-    _check_rms(x, weight, residual, eps)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return RMSNormFunction.apply(x, weight, eps, residual)
-    y, h, _, _ = _rms_fwd(x, weight, eps, residual, True, False, None)
+    y, h, _, _, _ = _row_call(_lib.row_ops().rms_fwd, x, x, weight, eps, residual, True, False, -1)
     return y if residual is None else (y, h)
 
 
@@ -1499,182 +1351,63 @@ def rms_norm_f8(x, weight=None, eps=1e-6, residual=None, dtype=torch.float8_e4m3
     """rms_norm of the rows x [R, C] straight to 8-bit rows (``f8_rows`` of the unrounded result,
     which itself is not written): -> (F8Rows, h), h = x without a residual.  For serving: no
     gradient flows through it."""
-    _check_rms(x, weight, residual, eps)
-    if x.dim() != 2:
-        raise ValueError("rms_norm_f8: x must be [rows, columns]")
-    if dtype not in _F8_CODE:
-        raise TypeError("rms_norm_f8: float8_e4m3fn or float8_e5m2")
-    _, h, _, q8 = _rms_fwd(x.detach(), weight, eps, residual, False, False, dtype)
-    return q8, h
+    _, h, _, data, scale = _row_call(_lib.row_ops().rms_fwd, x, x, weight, eps, residual, False,
+                                     False, _f8_code(dtype))
+    return F8Rows(data, scale), x.detach() if h is None else h
 
 
 # ------------------------------------------------------------------ 8-bit rows with block scales
 
-F8_BLOCK = 128
-
 # A matrix [R, C] in 8-bit form: data [R, C] float8 and scale float8_e8m0fnu, [R, ceil(C / 128)]
 # (one power of two for each 128 columns of a row) or [ceil(R / 128), ceil(C / 128)] (for each
 # 128 x 128: weights).  An element stands for data * scale.  Rows of data start on 16-byte borders
-# and rows of scale on 4-byte borders (the views below have such strides).
+# and rows of scale on 4-byte borders (the views that the functions below return have such strides).
 F8Rows = namedtuple("F8Rows", ["data", "scale"])
 
 
-def _f8_empty(rows, cols, scale_rows, dtype, device):
-    data = torch.empty((rows, -(-cols // 16) * 16), dtype=dtype, device=device)
-    nb = -(-cols // F8_BLOCK)
-    scale = torch.empty((scale_rows, -(-nb // 4) * 4), dtype=torch.float8_e8m0fnu, device=device)
-    return F8Rows(data[:, :cols], scale[:, :nb])
-
-
-def _f8_quant(x, dtype, square, rows, cols):
-    _need_cuda(x)
-    if x.dim() != 2:
-        raise ValueError(f"8-bit rows are made from a matrix, got {tuple(x.shape)}")
-    if x.dtype not in _TYPE_CODE:
-        raise TypeError(f"8-bit rows are made from float32, bfloat16 or float16, got {x.dtype}")
-    if dtype not in _F8_CODE:
-        raise TypeError("8-bit rows are float8_e4m3fn or float8_e5m2")
-    x = x.detach()
-    R, C = x.shape
-    if R >= 1 << 31 or C >= 1 << 31:
-        raise ValueError("8-bit rows: fewer than 2^31 rows and columns")
-    x, ldx = _rows2d(x, C)
-    L = _lib.lib()
-    with _on_device(x):
-        block = (lambda n: -(-n // F8_BLOCK)) if square else (lambda n: n)
-        q = _f8_empty(R, C, block(R), dtype, x.device) if rows else None
-        t = _f8_empty(C, R, block(C), dtype, x.device) if cols else None
-        a = (_ptr(q.data), q.data.stride(0), _ptr(q.scale), q.scale.stride(0)) if rows and R and C \
-            else (None, 0, None, 0)
-        b = (_ptr(t.data), t.data.stride(0), _ptr(t.scale), t.scale.stride(0)) if cols and R and C \
-            else (None, 0, None, 0)
-        check(L.lcf_f8_quant(_ptr(x), ldx, R, C, _TYPE_CODE[x.dtype], _F8_CODE[dtype],
-                             int(square), *a, *b, _stream()))
-    return q, t
-
-
 def f8_rows(x, dtype=torch.float8_e4m3fn):
-    """x [R, C] in 8-bit form, blocks of 128 along each row (what a product over C takes)."""
-    return _f8_quant(x, dtype, False, True, False)[0]
+    """x [R, C] (float32, bfloat16 or float16) in 8-bit form, blocks of 128 along each row (what a
+    product over C takes): q = round(x * 2^-e) to nearest even, 2^e the smallest power of two that
+    brings the block's largest finite magnitude inside the format; infinities and NaN become NaN.
+    include/lcf.h: lcf_f8_quant."""
+    return F8Rows(*_row_call(_lib.row_ops().f8_rows, x, x, _f8_code(dtype)))
 
 
 def f8_cols(x, dtype=torch.float8_e4m3fn):
     """x^T [C, R] in 8-bit form, blocks of 128 along each column of x (what a product over R -- a
     weight gradient -- takes)."""
-    return _f8_quant(x, dtype, False, False, True)[1]
+    return F8Rows(*_row_call(_lib.row_ops().f8_quant, x, x, _f8_code(dtype), False, False, True)[2:])
 
 
 def f8_rows_cols(x, dtype=torch.float8_e4m3fn):
     """(f8_rows(x), f8_cols(x)) from one reading of x."""
-    return _f8_quant(x, dtype, False, True, True)
+    r = _row_call(_lib.row_ops().f8_quant, x, x, _f8_code(dtype), False, True, True)
+    return F8Rows(*r[:2]), F8Rows(*r[2:])
 
 
 def f8_weight_image(weight, transpose=False, dtype=torch.float8_e4m3fn):
     """A weight [N, K] in 8-bit form with one scale for each 128 x 128; ``transpose``: the image of
     weight^T (the same bytes, turned: 128 x 128 blocks serve both directions)."""
-    q, t = _f8_quant(weight, dtype, True, not transpose, transpose)
-    return t if transpose else q
-
-
-def _f8_operand(m, name):
-    """Checks an F8Rows operand; rows that do not start on the borders the kernel reads from (a
-    tensor of the caller's own making) are copied once."""
-    try:
-        data, scale = m
-    except (TypeError, ValueError):
-        raise TypeError(f"f8_matmul: {name} must be (data, scale)") from None
-    _need_cuda(data, scale)
-    if data.dim() != 2 or scale.dim() != 2 or data.dtype not in _F8_CODE or scale.dtype not in (
-            torch.float8_e8m0fnu, torch.uint8):
-        raise TypeError(f"f8_matmul: {name} must be a float8 matrix and its E8M0 scales")
-    R, C = data.shape
-    nb = -(-C // F8_BLOCK)
-    if scale.shape[1] != nb or scale.shape[0] not in (R, -(-R // F8_BLOCK)):
-        raise ValueError(f"f8_matmul: {name} {tuple(data.shape)} needs scales "
-                         f"[{R} or {-(-R // F8_BLOCK)}, {nb}], got {tuple(scale.shape)}")
-    if data.get_device() != scale.get_device():
-        raise RuntimeError("f8_matmul: all tensors must be on one device")
-    return F8Rows(_bordered(data, 16), _bordered(scale, 4))
-
-
-def _bordered(t, to):
-    """t [R, C] of bytes with every row on a ``to``-byte border and readable up to the next one."""
-    R, C = t.shape
-    room = -(-C // to) * to
-    ld = t.stride(0) if R > 1 else room
-    if t.numel() == 0 or ((t.stride(1) == 1 or C == 1) and ld >= room and ld % to == 0
-                          and t.data_ptr() % to == 0 and t.untyped_storage().nbytes()
-                          >= t.storage_offset() + (R - 1) * ld + room):
-        return t
-    out = torch.zeros((R, room), dtype=torch.uint8, device=t.device)
-    out[:, :C] = t.view(torch.uint8)
-    return out.view(t.dtype)[:, :C]
+    r = _row_call(_lib.row_ops().f8_quant, weight, weight, _f8_code(dtype), True, not transpose,
+                  bool(transpose))
+    return F8Rows(*(r[2:] if transpose else r[:2]))
 
 
 def f8_matmul(a, b, scale=None, shift=None, relu=False, out_dtype=torch.float32, out=None):
     """out [M, N] = act((A B^T) * scale + shift) for A [M, K], B [N, K] in 8-bit form (F8Rows or
-    (data, scale) pairs; either with row or 128 x 128 scales for B, row scales for A), scale /
-    shift [N] float32 or None, act = max(x, 0) with ``relu``.  fp32 accumulation on the 8-bit
-    matrix cores; out_dtype float32, bfloat16 or float16.  ``out``: caller-owned [M, N] with unit
-    stride in a row.  include/lcf.h: lcf_f8_gemm."""
-    a, b = _f8_operand(a, "a"), _f8_operand(b, "b")
-    (M, K), (N, K2) = a.data.shape, b.data.shape
-    if K != K2:
-        raise ValueError(f"f8_matmul: {tuple(a.data.shape)} against {tuple(b.data.shape)}: the "
-                         "last dimensions must agree")
-    if a.scale.shape[0] != M:
-        raise ValueError("f8_matmul: a needs one scale for each row and 128 columns")
-    dev = a.data.device
-    for name, v in (("scale", scale), ("shift", shift)):
-        if v is not None and (v.dtype != torch.float32 or tuple(v.shape) != (N,)
-                              or not v.is_contiguous() or v.get_device() != a.data.get_device()):
-            raise ValueError(f"f8_matmul: {name} must be {N} contiguous float32 on the operands' device")
-    if b.data.get_device() != a.data.get_device():
-        raise RuntimeError("f8_matmul: all tensors must be on one device")
-    if out is not None:
-        if tuple(out.shape) != (M, N) or out.dtype not in _TYPE_CODE or not out.is_cuda or (
-                out.get_device() != a.data.get_device()) or (N > 1 and out.stride(1) != 1) or (
-                M > 1 and out.stride(0) < N):
-            raise ValueError(f"f8_matmul: out must be a float matrix [{M}, {N}] with unit stride "
-                             "in a row on the operands' device")
-    elif out_dtype not in _TYPE_CODE:
-        raise TypeError("f8_matmul: out_dtype must be float32, bfloat16 or float16")
-    L = _lib.lib()
-    with _on_device(a.data):
-        if out is None:
-            out = torch.empty((M, N), dtype=out_dtype, device=dev)
-        nbytes = L.lcf_f8_gemm_workspace_bytes(M, N, K, _TYPE_CODE[out.dtype])
-        ws = _ws(nbytes, dev) if nbytes else None
-        check(L.lcf_f8_gemm(
-            _ptr(a.data), a.data.stride(0) if M > 1 else -(-K // 16) * 16, _ptr(a.scale),
-            a.scale.stride(0) if M > 1 else -(-a.scale.shape[1] // 4) * 4, _F8_CODE[a.data.dtype],
-            _ptr(b.data), b.data.stride(0) if N > 1 else -(-K // 16) * 16, _ptr(b.scale),
-            b.scale.stride(0) if b.scale.shape[0] > 1 else -(-b.scale.shape[1] // 4) * 4,
-            _F8_CODE[b.data.dtype], int(b.scale.shape[0] != N), M, N, K, _ptr(scale), _ptr(shift),
-            int(bool(relu)), _ptr(out), out.stride(0) if M > 1 else N, _TYPE_CODE[out.dtype],
-            _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
-    return out
+    (data, scale) pairs; row scales for A, row or 128 x 128 scales for B), scale / shift [N]
+    float32 or None, act = max(x, 0) with ``relu``; out_dtype float32, bfloat16 or float16 (the
+    arithmetic goes by it, see include/lcf.h: lcf_f8_gemm).  Rows that do not start on the borders
+    the kernels read from are copied once.  ``out``: caller-owned [M, N] with unit stride in a
+    row."""
+    return _row_call(_lib.row_ops().f8_mm, a[0], a, b, scale, shift, relu,
+                     _TYPE_CODE.get(out_dtype, -1), out)
 
 
-def _f8_product(x, b, shift=None, scale=None, relu=False):
-    """f8_matmul(f8_rows(x), b) of x's own type: one launch where lcf_f8_linear takes the sizes
-    (thin layers over many rows), two elsewhere."""
-    M, K = x.shape
-    N = b.data.shape[0]
-    x, ldx = _rows2d(x.detach(), K)
-    thin = (M >= 4096 and N <= 256 and 0 < K <= (256 if x.dtype == torch.float32 else 512)
-            and K % 8 == 0 and x.data_ptr() % 4 == 0 and ldx * x.element_size() % 4 == 0
-            and ldx <= 1 << 22)
-    if not thin or b.data.dtype != torch.float8_e4m3fn:
-        return f8_matmul(f8_rows(x), b, scale, shift, relu, out_dtype=x.dtype)
-    with _on_device(x):
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-        check(_lib.lib().lcf_f8_linear(
-            _ptr(x), ldx, _TYPE_CODE[x.dtype], _ptr(b.data),
-            b.data.stride(0) if N > 1 else -(-K // 16) * 16, _ptr(b.scale), b.scale.stride(0) if
-            b.scale.shape[0] > 1 else 4, int(b.scale.shape[0] != N), M, N, K, _ptr(scale),
-            _ptr(shift), int(bool(relu)), _ptr(out), N, _TYPE_CODE[x.dtype], _stream()))
-    return out
+def f8_product(x, b, scale=None, shift=None, relu=False):
+    """f8_matmul(f8_rows(x), b, ...) of x's own type: one launch where lcf_f8_linear takes the sizes
+    (thin layers over many rows; the same bits), two elsewhere."""
+    return _row_call(_lib.row_ops().f8_product, x, x, b, scale, shift, relu)
 
 
 class F8LinearFunction(torch.autograd.Function):
@@ -1685,33 +1418,17 @@ class F8LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, turned, x8):
-        image = f8_weight_image(weight, transpose=turned)
-        shift = None if bias is None else bias.detach().float().contiguous()
-        if x8 is None:
-            y = _f8_product(x, image, shift)
-        else:
-            y = f8_matmul(x8, image, shift=shift, out_dtype=x.dtype)
         ctx.save_for_backward(x, weight)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.bias_type = None if bias is None else _TYPE_CODE[bias.dtype]
         ctx.turned = turned
-        return y
+        return _row_call(_lib.row_ops().f8_linear_fwd, x, x, weight, bias, turned, x8)
 
     @staticmethod
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
-        dy = dy.to(x.dtype)
-        dx = dw = db = None
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        rows, cols = _f8_quant(dy, torch.float8_e4m3fn, False, need_x, need_w) \
-            if need_x or need_w else (None, None)
-        if need_x:
-            dx = f8_matmul(rows, f8_weight_image(weight, transpose=not ctx.turned),
-                           out_dtype=x.dtype)
-        if need_w:
-            pair = (f8_cols(x), cols) if ctx.turned else (cols, f8_cols(x))
-            dw = f8_matmul(*pair, out_dtype=weight.dtype)
-        if ctx.bias_dtype is not None and ctx.needs_input_grad[2]:
-            db = dy.float().sum(0).to(ctx.bias_dtype)
+        need = ctx.needs_input_grad
+        dx, dw, db = _row_call(_lib.row_ops().f8_linear_bwd, x, dy, x, weight, ctx.turned, need[0],
+                               need[1], ctx.bias_type if need[2] else None)
         return dx, dw, db, None, None
 
 
@@ -1721,14 +1438,13 @@ def f8_linear(x, weight, bias=None, turned=False, x8=None):
     types).  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.
     Error of an operand: half a step of e4m3, 2^-4 of a value, plus 2^-10 of its block's scale for
     small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
-    _need_cuda(x, weight, bias)
     if x.dtype not in _TYPE_CODE or weight.dtype not in _TYPE_CODE or weight.dim() != 2 or \
             x.dim() < 1 or x.shape[-1] != weight.shape[0 if turned else 1]:
         raise ValueError(f"f8_linear: x {tuple(x.shape)} {x.dtype} against weight "
                          f"{tuple(weight.shape)} {weight.dtype}")
     n = weight.shape[1 if turned else 0]
-    if bias is not None and (tuple(bias.shape) != (n,) or not bias.dtype.is_floating_point):
-        raise ValueError(f"f8_linear: bias must have {n} elements")
+    if bias is not None and (tuple(bias.shape) != (n,) or bias.dtype not in _TYPE_CODE):
+        raise ValueError(f"f8_linear: bias must have {n} float elements")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x8 is not None and tuple(x8[0].shape) != tuple(x2.shape):
         raise ValueError("f8_linear: x8 must be the 8-bit form of x")

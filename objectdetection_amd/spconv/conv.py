@@ -175,7 +175,7 @@ class SparseConvolution(SparseModule):
         scale = None if scale is None else scale.float().contiguous()
         shift = None if shift is None else shift.float().contiguous()
         if f8 is None:
-            return ops._f8_product(x, self._weight_image("f8"), shift, scale, relu)
+            return ops.f8_product(x, self._weight_image("f8"), scale, shift, relu)
         return ops.f8_matmul(f8, self._weight_image("f8"), scale, shift, relu, out_dtype=x.dtype)
 
     def _inference_forward(self, x, rb, scale, shift, relu):

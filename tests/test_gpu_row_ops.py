@@ -155,7 +155,7 @@ def test_f8_matmul_many_rows(cuda, shape):
     for dtype in DTYPES:
         x = torch.nn.functional.pad(a.to(dtype).to(cuda), (1, 2))[:, 1:1 + K]
         want = ops.f8_matmul(ops.f8_rows(x), w, shift=shift, relu=True, out_dtype=dtype)
-        assert torch.equal(ops._f8_product(x, w, shift, relu=True), want)
+        assert torch.equal(ops.f8_product(x, w, shift=shift, relu=True), want)
 
 
 def test_f8_matmul_epilogue_and_out(cuda):

@@ -108,7 +108,7 @@ def test_abi_refuses_bad_8_bit_operands():
 
     def quant(x=4096, ldx=64, R=4, C=64, dt=0, fmt=0, sq=0, q=4096, ldq=64, s=4096, lds=4, qt=None, ldqt=0, st=None,
               ldst=0):
-        return L.lcf_f8_quant(x, ldx, R, C, dt, fmt, sq, q, ldq, s, lds, qt, ldqt, st, ldst, None)
+        return L.lcf_f8_quant(x, ldx, R, C, dt, fmt, sq, q, ldq, s, lds, qt, ldqt, st, ldst, None, None)
     for bad in (dict(x=None), dict(ldx=10), dict(R=-1), dict(C=-1), dict(dt=7), dict(fmt=2), dict(q=None),
                 dict(q=4104), dict(ldq=56), dict(ldq=48), dict(s=None), dict(s=4098), dict(lds=2),
                 dict(qt=4096), dict(qt=4096, ldqt=16, st=4096, ldst=3), dict(qt=4096, ldqt=8, st=4096, ldst=4)):
