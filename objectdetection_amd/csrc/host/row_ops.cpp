@@ -4,23 +4,28 @@
 // all there is: the same checks in Python took 15 to 40 us a call, and 80 us for a list of 78
 // gradients.  The library's functions are handed over by address (objectdetection_amd/_lib.py loads
 // it), so there is one liblcf in a process and nothing is linked against.
-// Every function takes the raw stream last and expects the tensors' device to be the current one.
+// Work goes to the current stream of the tensors' device, which is made the current one meanwhile.
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros.h>
+#include <ATen/ops/zeros_like.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 
 #include "../../../include/lcf.h"
 
 namespace {
 
-struct Err {
+// a refusal, with the Python exception it becomes (a std::exception: autograd's threads take no other)
+struct Err : std::runtime_error {
     PyObject *type;
-    std::string what;
+    Err(PyObject *t, const std::string &what) : std::runtime_error(what), type(t) {}
 };
-[[noreturn]] void fail(PyObject *type, std::string what) { throw Err{type, std::move(what)}; }
+[[noreturn]] void fail(PyObject *type, const std::string &what) { throw Err(type, what); }
 
 #define LCF_FUNCTIONS(F)                                                                                       \
     F(strerror) F(grad_norm_workspace_bytes) F(grad_norm) F(grad_clip) F(rms_norm_fwd) F(rms_norm_workspace_bytes) \
@@ -68,7 +73,6 @@ double real(PyObject *o)
     }
     return v;
 }
-void *stream_of(PyObject *o) { return PyLong_AsVoidPtr(o); }
 
 int type_code(at::ScalarType t)
 {
@@ -84,6 +88,12 @@ void on_gpu(const at::Tensor &t)
         fail(PyExc_RuntimeError, "objectdetection_amd ops run on the GPU only (no CPU fallback); got a " +
                                      t.device().str() + " tensor");
 }
+// the device of x made current for a scope, and its current stream
+struct On {
+    c10::DeviceGuard guard;
+    void *st;
+    explicit On(const at::Tensor &x) : guard((on_gpu(x), x.device())), st(c10::hip::getCurrentHIPStream(x.get_device()).stream()) {}
+};
 void beside(const at::Tensor &t, const at::Tensor &x, const char *who)
 {
     on_gpu(t);
@@ -318,21 +328,28 @@ F8 weight_image(const at::Tensor &w, bool transpose, int fmt, void *st)
 
 // ---- entry points
 using Args = PyObject *const *;
-template <typename F> PyObject *guarded(Py_ssize_t got, Py_ssize_t want, F f)
+template <typename F> PyObject *guarded_grad(Py_ssize_t got, Py_ssize_t want, F f)
 {
     try {
         if (got != want) fail(PyExc_TypeError, "wrong number of arguments");
         if (!L.strerror) fail(PyExc_RuntimeError, "row_ops: bind() first");
-        at::AutoDispatchBelowADInplaceOrView below; // nothing here is recorded by autograd
         return f();
     } catch (const Err &e) {
-        PyErr_SetString(e.type, e.what.c_str());
+        PyErr_SetString(e.type, e.what());
     } catch (const std::exception &e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     } catch (...) {
         PyErr_SetString(PyExc_RuntimeError, "row_ops: unknown error");
     }
     return nullptr;
+}
+
+template <typename F> PyObject *guarded(Py_ssize_t got, Py_ssize_t want, F f)
+{
+    return guarded_grad(got, want, [&] {
+        at::AutoDispatchBelowADInplaceOrView below; // nothing in here is recorded by autograd
+        return f();
+    });
 }
 
 PyObject *py_bind(PyObject *, Args a, Py_ssize_t n)
@@ -357,174 +374,258 @@ PyObject *py_bind(PyObject *, Args a, Py_ssize_t n)
     Py_RETURN_NONE;
 }
 
-// f8_quant(x, format, square, rows, cols, stream) -> (data, scale, data^T, scale^T)
-PyObject *py_f8_quant(PyObject *, Args a, Py_ssize_t n)
+// ---- the operators with their gradients
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Maybe = std::optional<Tensor>;
+const Tensor *maybe(const Maybe &t) { return t && t->defined() ? &*t : nullptr; }
+bool wants(const Tensor *t) { return t && t->requires_grad(); }
+
+struct Normed {
+    Tensor y, h, inv;
+    F8 q;
+};
+Normed rms_fwd(const Tensor &x, const Tensor *w, double eps, const Tensor *r, bool want_y, bool want_inv, int fmt)
 {
-    return guarded(n, 6, [&] {
-        const Quant q = f8_quant(need(a[0]), (int)number(a[1]), truth(a[2]), truth(a[3]), truth(a[4]), false, stream_of(a[5]));
-        return tuple(q.rows.data, q.rows.scale, q.cols.data, q.cols.scale);
-    });
+    const On on(x);
+    const int code = type_code(x.scalar_type());
+    if (code < 0 || x.dim() < 1) fail(PyExc_TypeError, "rms_norm: rows must be float32, bfloat16 or float16");
+    const long long width = x.size(-1);
+    if (width < 1 || width > 16384) fail(PyExc_ValueError, "rms_norm: 1 to 16384 columns, got " + std::to_string(width));
+    if (!(eps >= 0.0)) fail(PyExc_ValueError, "rms_norm: eps must not be negative");
+    Tensor wc;
+    if (w) {
+        beside(*w, x, "rms_norm");
+        if (type_code(w->scalar_type()) < 0 || w->dim() != 1 || w->size(0) != width)
+            fail(PyExc_ValueError, "rms_norm: weight must be a float tensor of " + std::to_string(width) + " elements");
+        wc = w->contiguous();
+    }
+    if (r) {
+        beside(*r, x, "rms_norm");
+        if (r->sizes() != x.sizes() || r->scalar_type() != x.scalar_type())
+            fail(PyExc_ValueError, "rms_norm: residual must have x's shape and type");
+    }
+    if (fmt >= 0 && x.dim() != 2) fail(PyExc_ValueError, "rms_norm_f8: x must be [rows, columns]");
+    const Rows v = rows_of(x, width), rv = r ? rows_of(*r, width) : Rows{Tensor(), 0, 0};
+    const int rows = count(v.n, "rms_norm");
+    Normed o;
+    if (want_y) o.y = at::empty(x.sizes(), x.options());
+    if (r) o.h = at::empty(x.sizes(), x.options());
+    if (want_inv) o.inv = at::empty({rows}, x.options().dtype(at::kFloat));
+    const bool q8 = fmt >= 0;
+    if (q8) o.q = f8_empty(rows, width, false, fmt, x);
+    check(L.rms_norm_fwd(v.ptr(), v.ld, r ? rv.ptr() : nullptr, rv.ld, rows, (int)width, code, w ? wc.data_ptr() : nullptr,
+                         w ? type_code(wc.scalar_type()) : 0, (float)eps, want_y ? o.y.data_ptr() : nullptr,
+                         r ? o.h.data_ptr() : nullptr, want_inv ? (float *)o.inv.data_ptr() : nullptr,
+                         q8 && rows ? o.q.q() : nullptr, o.q.ld, q8 && rows ? o.q.s() : nullptr, (int)o.q.lds, q8 ? fmt : 0,
+                         on.st));
+    return o;
 }
-// f8_rows(x, format, stream) -> (data, scale)
-PyObject *py_f8_rows(PyObject *, Args a, Py_ssize_t n)
-{
-    return guarded(n, 3, [&] {
-        const Quant q = f8_quant(need(a[0]), (int)number(a[1]), false, true, false, false, stream_of(a[2]));
-        return tuple(q.rows.data, q.rows.scale);
-    });
-}
-// f8_mm(a, b, scale, shift, relu, out type, out, stream)
-PyObject *py_f8_mm(PyObject *, Args a, Py_ssize_t n)
-{
-    return guarded(n, 8, [&] {
-        return wrap(f8_mm(f8_operand(a[0], "a"), f8_operand(a[1], "b"), maybe(a[2]), maybe(a[3]), truth(a[4]),
-                          (int)number(a[5]), maybe(a[6]), stream_of(a[7])));
-    });
-}
-// f8_product(x, b, scale, shift, relu, stream)
-PyObject *py_f8_product(PyObject *, Args a, Py_ssize_t n)
-{
-    return guarded(n, 6, [&] {
-        return wrap(f8_product(need(a[0]), f8_operand(a[1], "b"), maybe(a[2]), maybe(a[3]), truth(a[4]), stream_of(a[5])));
-    });
-}
-// f8_linear_fwd(x, weight, bias, turned, x8, stream) -> y
-PyObject *py_f8_linear_fwd(PyObject *, Args a, Py_ssize_t n)
-{
-    return guarded(n, 6, [&] {
-        const at::Tensor &x = need(a[0]), &w = need(a[1]);
-        on_gpu(x);
-        beside(w, x, "f8_linear");
-        void *st = stream_of(a[5]);
-        const F8 image = weight_image(w, truth(a[3]), LCF_E4M3, st);
-        at::Tensor shift;
-        if (const at::Tensor *b = maybe(a[2])) {
-            beside(*b, x, "f8_linear");
-            shift = b->to(at::kFloat).contiguous();
+
+// y (and h = x + residual) from x; backward from h and the rows' inverse root mean squares.  x and the
+// residual share one gradient.
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Maybe &w, double eps, const Maybe &r)
+    {
+        const Normed o = rms_fwd(x, maybe(w), eps, maybe(r), true, true, -1);
+        ctx->saved_data["two"] = maybe(r) != nullptr;
+        ctx->save_for_backward({maybe(r) ? o.h : x, w ? *w : Tensor(), o.inv});
+        ctx->set_materialize_grads(false);
+        if (maybe(r)) return {o.y, o.h};
+        return {o.y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const variable_list saved = ctx->get_saved_variables();
+        const bool two = ctx->saved_data["two"].toBool();
+        const Tensor &h = saved[0], &w = saved[1];
+        const bool need_w = w.defined() && ctx->needs_input_grad(1);
+        Tensor dy = grads[0], dh = two ? grads[1] : Tensor();
+        if (!dy.defined()) { // the norm's output was not used: the sum's gradient passes through
+            return {dh, need_w && dh.defined() ? at::zeros_like(w) : Tensor(), Tensor(), two ? dh : Tensor()};
         }
-        const at::Tensor *sh = shift.defined() ? &shift : nullptr;
-        if (a[4] == Py_None) return wrap(f8_product(x, image, nullptr, sh, false, st));
-        return wrap(f8_mm(f8_operand(a[4], "x8"), image, nullptr, sh, false, type_code(x.scalar_type()), nullptr, st));
-    });
-}
-// f8_linear_bwd(dy, x, weight, turned, need dx, need dw, bias type or None, stream) -> (dx, dw, db)
-PyObject *py_f8_linear_bwd(PyObject *, Args a, Py_ssize_t n)
+        const On on(h);
+        const long long width = h.size(-1);
+        if (dy.scalar_type() != h.scalar_type()) dy = dy.to(h.scalar_type());
+        if (dh.defined() && dh.scalar_type() != h.scalar_type()) dh = dh.to(h.scalar_type());
+        const Rows hv = rows_of(h, width), dv = rows_of(dy, width),
+                   gv = dh.defined() ? rows_of(dh, width) : Rows{Tensor(), 0, 0};
+        const int rows = count(hv.n, "rms_norm"), code = type_code(h.scalar_type());
+        Tensor dx = at::empty(h.sizes(), h.options()), dw, ws, wc;
+        if (w.defined()) wc = w.contiguous();
+        if (need_w) {
+            dw = at::empty({width}, w.options());
+            ws = bytes(L.rms_norm_workspace_bytes(rows, (int)width), h);
+        }
+        check(L.rms_norm_bwd(hv.ptr(), hv.ld, dv.ptr(), dv.ld, dh.defined() ? gv.ptr() : nullptr, gv.ld, rows, (int)width,
+                             code, w.defined() ? wc.data_ptr() : nullptr, w.defined() ? type_code(wc.scalar_type()) : 0,
+                             (const float *)saved[2].data_ptr(), dx.data_ptr(), need_w ? dw.data_ptr() : nullptr,
+                             need_w ? ws.data_ptr() : nullptr, need_w ? (size_t)ws.numel() : 0, on.st));
+        return {dx, dw, Tensor(), two ? dx : Tensor()};
+    }
+};
+
+Tensor f8_linear_fwd(const Tensor &x, const Tensor &w, const Tensor *bias, bool turned, const F8 *x8)
 {
-    return guarded(n, 8, [&] {
-        const at::Tensor &x = need(a[1]), &w = need(a[2]);
-        const bool turned = truth(a[3]), need_x = truth(a[4]), need_w = truth(a[5]), need_b = a[6] != Py_None;
-        void *st = stream_of(a[7]);
-        at::Tensor dy = need(a[0]);
-        beside(dy, x, "f8_linear");
+    const On on(x);
+    beside(w, x, "f8_linear");
+    const F8 image = weight_image(w, turned, LCF_E4M3, on.st);
+    Tensor shift;
+    if (bias) {
+        beside(*bias, x, "f8_linear");
+        shift = bias->to(at::kFloat).contiguous();
+    }
+    const Tensor *sh = bias ? &shift : nullptr;
+    if (!x8) return f8_product(x, image, nullptr, sh, false, on.st);
+    return f8_mm(*x8, image, nullptr, sh, false, type_code(x.scalar_type()), nullptr, on.st);
+}
+
+// y = x W^T (+ bias) with x and W rounded to 8-bit form.  The three products (y, dx = dy W, dW = dy^T x)
+// run on 8-bit operands, each operand's scale blocks lying along the axis that its product sums over;
+// the rounding is passed through unchanged.  turned: the weight is stored [K, N].
+struct F8Linear : torch::autograd::Function<F8Linear> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Maybe &bias, bool turned,
+                          const F8 *x8)
+    {
+        ctx->save_for_backward({x, w});
+        ctx->saved_data["turned"] = turned;
+        ctx->saved_data["bias"] = (int64_t)(maybe(bias) ? type_code(bias->scalar_type()) : -1);
+        return f8_linear_fwd(x, w, maybe(bias), turned, x8);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1];
+        const bool turned = ctx->saved_data["turned"].toBool();
+        const int bias = (int)ctx->saved_data["bias"].toInt();
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
+                   need_b = bias >= 0 && ctx->needs_input_grad(2);
+        const On on(x);
+        Tensor dy = grads[0], dx, dw, db;
         if (dy.scalar_type() != x.scalar_type()) dy = dy.to(x.scalar_type());
-        at::Tensor dx, dw, db;
         // the input's gradient takes dy as it is where one launch does both; elsewhere dy's rows form, its
         // columns form and the bias's sums come out of one reading
         F8 image;
         if (need_x) {
-            image = weight_image(w, !turned, LCF_E4M3, st);
-            dx = f8_fused(dy, image, nullptr, nullptr, false, st);
+            image = weight_image(w, !turned, LCF_E4M3, on.st);
+            dx = f8_fused(dy, image, nullptr, nullptr, false, on.st);
         }
         const bool rows = need_x && !dx.defined();
         Quant q;
-        if (rows || need_w || need_b) q = f8_quant(dy, LCF_E4M3, false, rows, need_w, need_b, st);
-        if (rows) dx = f8_mm(q.rows, image, nullptr, nullptr, false, type_code(dy.scalar_type()), nullptr, st);
+        if (rows || need_w || need_b) q = f8_quant(dy, LCF_E4M3, false, rows, need_w, need_b, on.st);
+        if (rows) dx = f8_mm(q.rows, image, nullptr, nullptr, false, type_code(dy.scalar_type()), nullptr, on.st);
         if (need_w) {
-            const F8 xt = f8_quant(x, LCF_E4M3, false, false, true, false, st).cols;
+            const F8 xt = f8_quant(x, LCF_E4M3, false, false, true, false, on.st).cols;
             dw = f8_mm(turned ? xt : q.cols, turned ? q.cols : xt, nullptr, nullptr, false, type_code(w.scalar_type()),
-                       nullptr, st);
+                       nullptr, on.st);
         }
         if (need_b) {
-            const int code = (int)number(a[6]);
             const int C = (int)dy.size(1);
-            db = at::empty({C}, dy.options().dtype(type_of(code)));
-            if (C) check(L.sum_parts((const float *)q.sums.data_ptr(), (int)q.sums.size(0), C, db.data_ptr(), code, st));
+            db = at::empty({C}, dy.options().dtype(type_of(bias)));
+            if (C) check(L.sum_parts((const float *)q.sums.data_ptr(), (int)q.sums.size(0), C, db.data_ptr(), bias, on.st));
         }
-        return tuple(dx, dw, db);
-    });
-}
+        return {dx, dw, db, Tensor(), Tensor()};
+    }
+};
 
-// rms_fwd(x, weight, eps, residual, want y, want inv, 8-bit format or -1, stream)
-//   -> (y, h, inv, data, scale); h is None without a residual
-PyObject *py_rms_fwd(PyObject *, Args a, Py_ssize_t n)
-{
-    return guarded(n, 8, [&] {
-        const at::Tensor &x = need(a[0]);
-        const at::Tensor *w = maybe(a[1]), *r = maybe(a[3]);
-        const double eps = real(a[2]);
-        const int fmt = (int)number(a[6]), code = type_code(x.scalar_type());
-        on_gpu(x);
-        if (code < 0 || x.dim() < 1) fail(PyExc_TypeError, "rms_norm: rows must be float32, bfloat16 or float16");
-        const long long width = x.size(-1);
-        if (width < 1 || width > 16384)
-            fail(PyExc_ValueError, "rms_norm: 1 to 16384 columns, got " + std::to_string(width));
-        if (!(eps >= 0.0)) fail(PyExc_ValueError, "rms_norm: eps must not be negative");
-        at::Tensor wc;
-        if (w) {
-            beside(*w, x, "rms_norm");
-            if (type_code(w->scalar_type()) < 0 || w->dim() != 1 || w->size(0) != width)
-                fail(PyExc_ValueError, "rms_norm: weight must be a float tensor of " + std::to_string(width) + " elements");
-            wc = w->contiguous();
-        }
-        if (r) {
-            beside(*r, x, "rms_norm");
-            if (r->sizes() != x.sizes() || r->scalar_type() != x.scalar_type())
-                fail(PyExc_ValueError, "rms_norm: residual must have x's shape and type");
-        }
-        if (fmt >= 0 && x.dim() != 2) fail(PyExc_ValueError, "rms_norm_f8: x must be [rows, columns]");
-        const Rows v = rows_of(x, width), rv = r ? rows_of(*r, width) : Rows{at::Tensor(), 0, 0};
-        const int rows = count(v.n, "rms_norm");
-        at::Tensor y, h, inv;
-        if (truth(a[4])) y = at::empty(x.sizes(), x.options());
-        if (r) h = at::empty(x.sizes(), x.options());
-        if (truth(a[5])) inv = at::empty({rows}, x.options().dtype(at::kFloat));
-        F8 q;
-        if (fmt >= 0) q = f8_empty(rows, width, false, fmt, x);
-        check(L.rms_norm_fwd(v.ptr(), v.ld, r ? rv.ptr() : nullptr, rv.ld, rows, (int)width, code,
-                             w ? wc.data_ptr() : nullptr, w ? type_code(wc.scalar_type()) : 0, (float)eps,
-                             y.defined() ? y.data_ptr() : nullptr, r ? h.data_ptr() : nullptr,
-                             inv.defined() ? (float *)inv.data_ptr() : nullptr, fmt >= 0 && rows ? q.q() : nullptr, q.ld,
-                             fmt >= 0 && rows ? q.s() : nullptr, (int)q.lds, fmt >= 0 ? fmt : 0, stream_of(a[7])));
-        return tuple(y, h, inv, q.data, q.scale);
-    });
-}
-// rms_bwd(h, weight, inv, dy, dh, need dw, stream) -> (dx, dw)
-PyObject *py_rms_bwd(PyObject *, Args a, Py_ssize_t n)
-{
-    return guarded(n, 7, [&] {
-        const at::Tensor &h = need(a[0]), &inv = need(a[2]);
-        const at::Tensor *w = maybe(a[1]), *g = maybe(a[4]);
-        at::Tensor dy = need(a[3]), dh;
-        const long long width = h.size(-1);
-        const int code = type_code(h.scalar_type());
-        beside(dy, h, "rms_norm");
-        if (dy.sizes() != h.sizes()) fail(PyExc_ValueError, "rms_norm: a gradient of another shape");
-        if (dy.scalar_type() != h.scalar_type()) dy = dy.to(h.scalar_type());
-        if (g) {
-            beside(*g, h, "rms_norm");
-            if (g->sizes() != h.sizes()) fail(PyExc_ValueError, "rms_norm: a gradient of another shape");
-            dh = g->scalar_type() == h.scalar_type() ? *g : g->to(h.scalar_type());
-        }
-        const Rows hv = rows_of(h, width), dv = rows_of(dy, width), gv = g ? rows_of(dh, width) : Rows{at::Tensor(), 0, 0};
-        const int rows = count(hv.n, "rms_norm");
-        at::Tensor dx = at::empty(h.sizes(), h.options()), dw, ws, wc;
-        if (w) wc = w->contiguous();
-        if (w && truth(a[5])) {
-            dw = at::empty({width}, w->options());
-            ws = bytes(L.rms_norm_workspace_bytes(rows, (int)width), h);
-        }
-        check(L.rms_norm_bwd(hv.ptr(), hv.ld, dv.ptr(), dv.ld, g ? gv.ptr() : nullptr, gv.ld, rows, (int)width, code,
-                             w ? wc.data_ptr() : nullptr, w ? type_code(wc.scalar_type()) : 0, (const float *)inv.data_ptr(),
-                             dx.data_ptr(), dw.defined() ? dw.data_ptr() : nullptr, ws.defined() ? ws.data_ptr() : nullptr,
-                             ws.defined() ? (size_t)ws.numel() : 0, stream_of(a[6])));
-        return tuple(dx, dw);
-    });
-}
-
-// clip(tensors, out or None, p, max_norm or None, stream) -> norm.  max_norm None: the norm alone.
-PyObject *py_clip(PyObject *, Args a, Py_ssize_t n)
+// f8_quant(x, format, square, rows, cols) -> (data, scale, data^T, scale^T)
+PyObject *py_f8_quant(PyObject *, Args a, Py_ssize_t n)
 {
     return guarded(n, 5, [&] {
+        const Tensor &x = need(a[0]);
+        const On on(x);
+        const Quant q = f8_quant(x, (int)number(a[1]), truth(a[2]), truth(a[3]), truth(a[4]), false, on.st);
+        return tuple(q.rows.data, q.rows.scale, q.cols.data, q.cols.scale);
+    });
+}
+// f8_rows(x, format) -> (data, scale)
+PyObject *py_f8_rows(PyObject *, Args a, Py_ssize_t n)
+{
+    return guarded(n, 2, [&] {
+        const Tensor &x = need(a[0]);
+        const On on(x);
+        const Quant q = f8_quant(x, (int)number(a[1]), false, true, false, false, on.st);
+        return tuple(q.rows.data, q.rows.scale);
+    });
+}
+// f8_mm(a, b, scale, shift, relu, out type, out)
+PyObject *py_f8_mm(PyObject *, Args a, Py_ssize_t n)
+{
+    return guarded(n, 7, [&] {
+        const F8 x = f8_operand(a[0], "a"), b = f8_operand(a[1], "b");
+        const On on(x.data);
+        return wrap(f8_mm(x, b, maybe(a[2]), maybe(a[3]), truth(a[4]), (int)number(a[5]), maybe(a[6]), on.st));
+    });
+}
+// f8_product(x, b, scale, shift, relu)
+PyObject *py_f8_product(PyObject *, Args a, Py_ssize_t n)
+{
+    return guarded(n, 5, [&] {
+        const Tensor &x = need(a[0]);
+        const On on(x);
+        return wrap(f8_product(x, f8_operand(a[1], "b"), maybe(a[2]), maybe(a[3]), truth(a[4]), on.st));
+    });
+}
+// f8_linear(x, weight, bias, turned, x8) -> y, differentiable
+PyObject *py_f8_linear(PyObject *, Args a, Py_ssize_t n)
+{
+    return guarded_grad(n, 5, [&] {
+        const Tensor &x = need(a[0]), &w = need(a[1]);
+        const Tensor *bias = maybe(a[2]);
+        const bool turned = truth(a[3]);
+        on_gpu(x);
+        if (type_code(x.scalar_type()) < 0 || type_code(w.scalar_type()) < 0 || x.dim() != 2 || w.dim() != 2 ||
+            x.size(1) != w.size(turned ? 0 : 1))
+            fail(PyExc_ValueError, "f8_linear: x " + shape(x) + " against weight " + shape(w) +
+                                       " (float32, bfloat16 or float16)");
+        const long long out = w.size(turned ? 1 : 0);
+        if (bias && (bias->dim() != 1 || bias->size(0) != out || type_code(bias->scalar_type()) < 0))
+            fail(PyExc_ValueError, "f8_linear: bias must have " + std::to_string(out) + " float elements");
+        F8 x8;
+        if (a[4] != Py_None) {
+            x8 = f8_operand(a[4], "x8");
+            if (x8.R != x.size(0) || x8.C != x.size(1)) fail(PyExc_ValueError, "f8_linear: x8 must be the 8-bit form of x");
+        }
+        const F8 *p8 = a[4] != Py_None ? &x8 : nullptr;
+        if (at::GradMode::is_enabled() && (wants(&x) || wants(&w) || wants(bias)))
+            return wrap(F8Linear::apply(x, w, bias ? Maybe(*bias) : Maybe(), turned, p8));
+        at::AutoDispatchBelowADInplaceOrView below;
+        return wrap(f8_linear_fwd(x, w, bias, turned, p8));
+    });
+}
+// rms_norm(x, weight, eps, residual) -> y, or (y, h) with a residual; differentiable
+PyObject *py_rms_norm(PyObject *, Args a, Py_ssize_t n)
+{
+    return guarded_grad(n, 4, [&]() -> PyObject * {
+        const Tensor &x = need(a[0]);
+        const Tensor *w = maybe(a[1]), *r = maybe(a[3]);
+        const double eps = real(a[2]);
+        on_gpu(x);
+        if (at::GradMode::is_enabled() && (wants(&x) || wants(w) || wants(r))) {
+            const variable_list o = RmsNorm::apply(x, w ? Maybe(*w) : Maybe(), eps, r ? Maybe(*r) : Maybe());
+            return r ? tuple(o[0], o[1]) : wrap(o[0]);
+        }
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Normed o = rms_fwd(x, w, eps, r, true, false, -1);
+        return r ? tuple(o.y, o.h) : wrap(o.y);
+    });
+}
+// rms_norm_f8(x, weight, eps, residual, format) -> (data, scale, h); h is None without a residual
+PyObject *py_rms_norm_f8(PyObject *, Args a, Py_ssize_t n)
+{
+    return guarded(n, 5, [&] {
+        const Normed o = rms_fwd(need(a[0]), maybe(a[1]), real(a[2]), maybe(a[3]), false, false, (int)number(a[4]));
+        return tuple(o.q.data, o.q.scale, o.h);
+    });
+}
+
+// clip(tensors, out or None, p, max_norm or None) -> norm.  max_norm None: the norm alone.
+PyObject *py_clip(PyObject *, Args a, Py_ssize_t n)
+{
+    return guarded(n, 4, [&] {
         if (!PyList_Check(a[0])) fail(PyExc_TypeError, "expected a list of tensors");
         const Py_ssize_t k = PyList_GET_SIZE(a[0]);
         if (k == 0) fail(PyExc_ValueError, "expected at least one tensor");
@@ -532,7 +633,7 @@ PyObject *py_clip(PyObject *, Args a, Py_ssize_t n)
         if (list && PyList_GET_SIZE(a[1]) != k) fail(PyExc_ValueError, "out must have a tensor for each gradient");
         std::vector<lcf_grad> t((size_t)k);
         const at::Tensor &first = need(PyList_GET_ITEM(a[0], 0));
-        on_gpu(first);
+        const On on(first);
         long long total = 0;
         auto take = [&](PyObject *o, const char *what) -> const at::Tensor & {
             const at::Tensor &g = need(o);
@@ -578,18 +679,17 @@ PyObject *py_clip(PyObject *, Args a, Py_ssize_t n)
         at::Tensor ws = bytes(L.grad_norm_workspace_bytes((int)k), first);
         if (clip)
             check(L.grad_clip(t.data(), (int)k, (int)number(a[2]), (float)real(a[3]), (float *)norm.data_ptr(),
-                              ws.data_ptr(), (size_t)ws.numel(), stream_of(a[4])));
+                              ws.data_ptr(), (size_t)ws.numel(), on.st));
         else
             check(L.grad_norm(t.data(), (int)k, (int)number(a[2]), (float *)norm.data_ptr(), ws.data_ptr(),
-                              (size_t)ws.numel(), stream_of(a[4])));
+                              (size_t)ws.numel(), on.st));
         return wrap(norm);
     });
 }
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)())py_##name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind),          METHOD(f8_quant),      METHOD(f8_rows), METHOD(f8_mm),   METHOD(f8_product),
-                         METHOD(f8_linear_fwd), METHOD(f8_linear_bwd), METHOD(rms_fwd), METHOD(rms_bwd), METHOD(clip),
-                         {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(bind),      METHOD(f8_quant), METHOD(f8_rows),     METHOD(f8_mm), METHOD(f8_product),
+                         METHOD(f8_linear), METHOD(rms_norm), METHOD(rms_norm_f8), METHOD(clip),  {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_row_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 } // namespace

@@ -1247,17 +1247,6 @@ _F8_CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}  # LCF_E4M3, LCF_E5M2
 _NORM_CODE = {1: 1, 1.0: 1, 2: 2, 2.0: 2, float("inf"): 0}
 
 
-def _row_call(fn, t, *args):
-    """fn(*args, stream) of the row operators' host module on the device of ``t`` (kernels go to that
-    device's current stream)."""
-    index = t.get_device() if isinstance(t, torch.Tensor) else -1
-    if index < 0 or index == torch.cuda.current_device():
-        # a tensor off the GPU is refused by fn itself, before any launch
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index) if index >= 0 else 0)
-    with torch.cuda.device(index):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
-
-
 def _f8_code(dtype):
     try:
         return _F8_CODE[dtype]
@@ -1274,7 +1263,7 @@ def grad_norm(tensors, norm_type=2.0):
     tensors = list(tensors)
     if not tensors:
         return torch.zeros(())
-    return _row_call(_lib.row_ops().clip, tensors[0], tensors, None, _NORM_CODE[norm_type], None)
+    return _lib.row_ops().clip(tensors, None, _NORM_CODE[norm_type], None)
 
 
 def clip_norm_(tensors, max_norm, norm_type=2.0, out=None):
@@ -1297,7 +1286,7 @@ def clip_norm_(tensors, max_norm, norm_type=2.0, out=None):
                                                        else out)):
             raise ValueError("out must have a tensor for each gradient")
         return torch.zeros(())
-    return _row_call(_lib.row_ops().clip, tensors[0], tensors, out, _NORM_CODE[norm_type], max_norm)
+    return _lib.row_ops().clip(tensors, out, _NORM_CODE[norm_type], max_norm)
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
@@ -1310,49 +1299,20 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
 
 # ------------------------------------------------------------------ RMS norm of rows
 
-class RMSNormFunction(torch.autograd.Function):
-    """(y, h) = RMS norm of x (+ residual); backward by lcf_rms_norm_bwd from h and the rows'
-    inverse root mean squares.  x and residual share one gradient."""
-
-    @staticmethod
-    def forward(ctx, x, weight, eps, residual):
-        y, h, inv, _, _ = _row_call(_lib.row_ops().rms_fwd, x, x, weight, eps, residual, True, True,
-                                    -1)
-        ctx.save_for_backward(x if h is None else h, weight, inv)
-        ctx.two = h is not None
-        ctx.set_materialize_grads(False)
-        return (y, h) if ctx.two else y
-
-    @staticmethod
-    def backward(ctx, dy, dh=None):
-        h, weight, inv = ctx.saved_tensors
-        need_w = weight is not None and ctx.needs_input_grad[1]
-        if dy is None:  # the norm's output was not used: the sum's gradient passes through
-            dw = torch.zeros_like(weight) if need_w and dh is not None else None
-            return dh, dw, None, dh if ctx.two else None
-        dx, dw = _row_call(_lib.row_ops().rms_bwd, h, h, weight, inv, dy, dh, need_w)
-        return dx, dw, None, dx if ctx.two else None
-
-
 def rms_norm(x, weight=None, eps=1e-6, residual=None):
     """Root-mean-square norm of the last dimension (1 to 16384 columns; float32, bfloat16 or
     float16; a row may start anywhere): y = h / sqrt(mean(h^2) + eps) * weight.  With ``residual``
     h = x + residual rounded to the rows' type, and (y, h) is returned; without it h = x and y is.
     Sums are held in 32 bits.  Differentiable in x, weight and residual.  include/lcf.h:
     lcf_rms_norm_fwd / _bwd."""
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        return RMSNormFunction.apply(x, weight, eps, residual)
-    y, h, _, _, _ = _row_call(_lib.row_ops().rms_fwd, x, x, weight, eps, residual, True, False, -1)
-    return y if residual is None else (y, h)
+    return _lib.row_ops().rms_norm(x, weight, eps, residual)
 
 
 def rms_norm_f8(x, weight=None, eps=1e-6, residual=None, dtype=torch.float8_e4m3fn):
     """rms_norm of the rows x [R, C] straight to 8-bit rows (``f8_rows`` of the unrounded result,
     which itself is not written): -> (F8Rows, h), h = x without a residual.  For serving: no
     gradient flows through it."""
-    _, h, _, data, scale = _row_call(_lib.row_ops().rms_fwd, x, x, weight, eps, residual, False,
-                                     False, _f8_code(dtype))
+    data, scale, h = _lib.row_ops().rms_norm_f8(x, weight, eps, residual, _f8_code(dtype))
     return F8Rows(data, scale), x.detach() if h is None else h
 
 
@@ -1370,26 +1330,25 @@ def f8_rows(x, dtype=torch.float8_e4m3fn):
     product over C takes): q = round(x * 2^-e) to nearest even, 2^e the smallest power of two that
     brings the block's largest finite magnitude inside the format; infinities and NaN become NaN.
     include/lcf.h: lcf_f8_quant."""
-    return F8Rows(*_row_call(_lib.row_ops().f8_rows, x, x, _f8_code(dtype)))
+    return F8Rows(*_lib.row_ops().f8_rows(x, _f8_code(dtype)))
 
 
 def f8_cols(x, dtype=torch.float8_e4m3fn):
     """x^T [C, R] in 8-bit form, blocks of 128 along each column of x (what a product over R -- a
     weight gradient -- takes)."""
-    return F8Rows(*_row_call(_lib.row_ops().f8_quant, x, x, _f8_code(dtype), False, False, True)[2:])
+    return F8Rows(*_lib.row_ops().f8_quant(x, _f8_code(dtype), False, False, True)[2:])
 
 
 def f8_rows_cols(x, dtype=torch.float8_e4m3fn):
     """(f8_rows(x), f8_cols(x)) from one reading of x."""
-    r = _row_call(_lib.row_ops().f8_quant, x, x, _f8_code(dtype), False, True, True)
+    r = _lib.row_ops().f8_quant(x, _f8_code(dtype), False, True, True)
     return F8Rows(*r[:2]), F8Rows(*r[2:])
 
 
 def f8_weight_image(weight, transpose=False, dtype=torch.float8_e4m3fn):
     """A weight [N, K] in 8-bit form with one scale for each 128 x 128; ``transpose``: the image of
     weight^T (the same bytes, turned: 128 x 128 blocks serve both directions)."""
-    r = _row_call(_lib.row_ops().f8_quant, weight, weight, _f8_code(dtype), True, not transpose,
-                  bool(transpose))
+    r = _lib.row_ops().f8_quant(weight, _f8_code(dtype), True, not transpose, bool(transpose))
     return F8Rows(*(r[2:] if transpose else r[:2]))
 
 
@@ -1400,53 +1359,23 @@ def f8_matmul(a, b, scale=None, shift=None, relu=False, out_dtype=torch.float32,
     arithmetic goes by it, see include/lcf.h: lcf_f8_gemm).  Rows that do not start on the borders
     the kernels read from are copied once.  ``out``: caller-owned [M, N] with unit stride in a
     row."""
-    return _row_call(_lib.row_ops().f8_mm, a[0], a, b, scale, shift, relu,
-                     _TYPE_CODE.get(out_dtype, -1), out)
+    return _lib.row_ops().f8_mm(a, b, scale, shift, relu, _TYPE_CODE.get(out_dtype, -1), out)
 
 
 def f8_product(x, b, scale=None, shift=None, relu=False):
     """f8_matmul(f8_rows(x), b, ...) of x's own type: one launch where lcf_f8_linear takes the sizes
     (thin layers over many rows; the same bits), two elsewhere."""
-    return _row_call(_lib.row_ops().f8_product, x, x, b, scale, shift, relu)
-
-
-class F8LinearFunction(torch.autograd.Function):
-    """y = x W^T (+ bias) with x and W rounded to 8-bit form; the three products (y, dx = dy W,
-    dW = dy^T x) run on 8-bit operands with fp32 accumulation, each operand's scale blocks lying
-    along the axis that its product sums over.  The rounding is passed through unchanged.
-    ``turned``: the weight is stored [K, N], as sparse convs store it."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, turned, x8):
-        ctx.save_for_backward(x, weight)
-        ctx.bias_type = None if bias is None else _TYPE_CODE[bias.dtype]
-        ctx.turned = turned
-        return _row_call(_lib.row_ops().f8_linear_fwd, x, x, weight, bias, turned, x8)
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, weight = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = _row_call(_lib.row_ops().f8_linear_bwd, x, dy, x, weight, ctx.turned, need[0],
-                               need[1], ctx.bias_type if need[2] else None)
-        return dx, dw, db, None, None
+    return _lib.row_ops().f8_product(x, b, scale, shift, relu)
 
 
 def f8_linear(x, weight, bias=None, turned=False, x8=None):
     """x [..., K] (float32, bfloat16 or float16) times weight [N, K]^T (+ bias [N]) on 8-bit
     operands: -> [..., N] of x's type, differentiable in all three (weight and bias keep their own
-    types).  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.
+    types): y, dx = dy W and dW = dy^T x are products of 8-bit operands whose scale blocks lie along
+    the axis that the product sums over; the rounding is passed through unchanged.  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.
     Error of an operand: half a step of e4m3, 2^-4 of a value, plus 2^-10 of its block's scale for
     small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
-    if x.dtype not in _TYPE_CODE or weight.dtype not in _TYPE_CODE or weight.dim() != 2 or \
-            x.dim() < 1 or x.shape[-1] != weight.shape[0 if turned else 1]:
-        raise ValueError(f"f8_linear: x {tuple(x.shape)} {x.dtype} against weight "
-                         f"{tuple(weight.shape)} {weight.dtype}")
-    n = weight.shape[1 if turned else 0]
-    if bias is not None and (tuple(bias.shape) != (n,) or bias.dtype not in _TYPE_CODE):
-        raise ValueError(f"f8_linear: bias must have {n} float elements")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x8 is not None and tuple(x8[0].shape) != tuple(x2.shape):
-        raise ValueError("f8_linear: x8 must be the 8-bit form of x")
-    y = F8LinearFunction.apply(x2, weight, bias, bool(turned), x8)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+    if x.dim() == 2:
+        return _lib.row_ops().f8_linear(x, weight, bias, turned, x8)
+    y = _lib.row_ops().f8_linear(x.reshape(-1, x.shape[-1]), weight, bias, turned, x8)
+    return y.view(*x.shape[:-1], y.shape[1])
