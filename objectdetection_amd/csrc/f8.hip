@@ -461,21 +461,22 @@ __global__ void __launch_bounds__(WM *WN * 64) f8_gemm_kernel(F8Gemm p)
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[i][t] = (f8_f4){0.f, 0.f, 0.f, 0.f};
     const int nb = f8_column<WIDE>(0, r16); // this lane's row of b in piece 0 of the wave
-    // scale words, four steps to a word, go through LDS as well: one word a thread (there are as many
-    // threads as rows of a and b), twice
-    static_assert(NT == BM + BN, "a thread for each row's scales");
+    // scale words, four steps to a word, go through LDS as well: one word a thread for each row of a and
+    // b, twice
+    static_assert(NT >= BM + BN && (BM + BN) % 64 == 0, "a thread for each row's scales, in whole waves");
     unsigned *ls = (unsigned *)(smem + 2 * (BM + BN) * 128);
     const unsigned char *srow =
         tid < BM ? p.sa + (long long)min(m0 + tid, p.M - 1) * p.ldsa
                  : p.sb + (long long)(min(n0 + tid - BM, p.N - 1) >> p.b_shift) * p.ldsb;
     auto load_scales = [&](int word) {
+        if (NT > BM + BN && wave >= (BM + BN) / 64) return;
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(srow + word * 4),
-                                         (__attribute__((address_space(3))) void *)(ls + (word & 1) * NT + wave * 64),
+                                         (__attribute__((address_space(3))) void *)(ls + (word & 1) * (BM + BN) + wave * 64),
                                          4, 0, 0);
     };
     unsigned xa[MT], xb[4];
     auto scales = [&](int step) {
-        const unsigned *l = ls + ((step >> 2) & 1) * NT;
+        const unsigned *l = ls + ((step >> 2) & 1) * (BM + BN);
         const int sh = (step & 3) * 8;
 #pragma unroll
         for (int i = 0; i < MT; ++i) xa[i] = l[wm + i * 16 + r16] >> sh;
@@ -814,6 +815,113 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
     }
 }
 
+// A few rows (M <= 64): bound by reading b once.  A workgroup takes 16 columns of the output, its waves
+// take turns of 512 bytes along k (four steps, one scale word): everything of a turn is asked for at
+// once, 8 KB of b a wave, straight into registers.  The waves' sums meet in LDS in a fixed order.
+// (Tiles of 128 rows leave a compute unit one 16 KB step in flight: 11.6 us and a join of 3.9 us at
+// 8 x 8192 x 4096.)
+template <int FA, int FB, bool WIDE, int MT> // (16 waves leave a wave 128 registers, which do for MT = 1)
+__global__ void __launch_bounds__(MT == 1 ? 1024 : 512) f8_few_kernel(F8Gemm p)
+{
+    extern __shared__ __align__(16) float few_sums[]; // [waves][MT][64][4]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int r16 = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, room = (p.K + 15) & ~15;
+    const __amdgpu_buffer_rsrc_t bbuf = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char *>(p.b + (long long)n0 * p.ldb), 0, (min(16, p.N - n0) - 1) * (int)p.ldb + room, 0x00020000);
+    const __amdgpu_buffer_rsrc_t abuf = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char *>(p.a), 0, (p.M - 1) * (int)p.lda + room, 0x00020000);
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    const unsigned char *sb = p.sb + (long long)(min(n0 + r16, p.N - 1) >> p.b_shift) * p.ldsb;
+    f8_f4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = (f8_f4){0.f, 0.f, 0.f, 0.f};
+    auto piece = [&](__amdgpu_buffer_rsrc_t buf, int row, int ld, int col) -> u4 {
+        return __builtin_amdgcn_raw_buffer_load_b128(buf, col < p.K ? row * ld + col : (int)0x80000000, 0, 0);
+    };
+    auto whole = [&](const u4 &lo, const u4 &hi, int col) -> f8_v8 {
+        int w[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { w[i] = (int)lo[i]; w[4 + i] = (int)hi[i]; }
+        if (p.K & 15) {
+            f8_cut(w, col, p.K);
+            f8_cut(w + 4, col + 64, p.K);
+        }
+        f8_v8 v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = w[i];
+        return v;
+    };
+    const int turns = (p.K + 511) >> 9;
+    for (int turn = wave; turn < turns; turn += waves) {
+        u4 b[4][2], a[MT][4][2];
+        unsigned xa[MT];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) b[k][h] = piece(bbuf, r16, (int)p.ldb, turn * 512 + k * 128 + g * 16 + h * 64);
+        const unsigned xb = *(const unsigned *)(sb + turn * 4);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int row = i * 16 + r16;
+            xa[i] = *(const unsigned *)(p.sa + (long long)min(row, p.M - 1) * p.ldsa + turn * 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    a[i][k][h] = piece(abuf, row, (int)p.lda, turn * 512 + k * 128 + g * 16 + h * 64);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int col = turn * 512 + k * 128 + g * 16;
+            if (turn * 512 + k * 128 >= p.K) break; // nothing of this step is there (its scale byte is not either)
+            const f8_v8 vb = whole(b[k][0], b[k][1], col);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const f8_v8 va = whole(a[i][k][0], a[i][k][1], col);
+                if constexpr (WIDE) {
+                    const float eb = lcf_exp2i((int)((xb >> (8 * k)) & 255) - 127);
+                    const float ea = lcf_exp2i((int)((xa[i] >> (8 * k)) & 255) - 127);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            f8_to_bf16<FB>(vb[2 * q], vb[2 * q + 1], eb), f8_to_bf16<FA>(va[2 * q], va[2 * q + 1], ea),
+                            acc[i], 0, 0, 0);
+                } else {
+                    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va, acc[i], FB, FA, 0,
+                                                                              (int)(xb >> (8 * k)), 0,
+                                                                              (int)(xa[i] >> (8 * k)));
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+        *reinterpret_cast<f8_f4 *>(few_sums + ((wave * MT + i) * 64 + lane) * 4) = acc[i];
+    __syncthreads();
+    // lane (r16, g) holds columns n0 + 4 g + r of row 16 i + r16
+    const int m = wave * 16 + r16, n = n0 + 4 * g;
+    if (wave >= MT || m >= p.M) return;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < waves; ++w) {
+        const f8_f4 q = *reinterpret_cast<const f8_f4 *>(few_sums + ((w * MT + wave) * 64 + lane) * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += q[r];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (n + r >= p.N) break;
+        float x = v[r];
+        if (p.scale) x *= p.scale[n + r];
+        if (p.shift) x += p.shift[n + r];
+        if (p.relu) x = x < 0.f ? 0.f : x;
+        const long long at = (long long)m * p.ldo + n + r;
+        if (p.code == LCF_F32) ((float *)p.out)[at] = x;
+        else if (p.code == LCF_BF16) ((lcf_b *)p.out)[at] = lcf_from_f32<lcf_b>(x);
+        else ((lcf_h *)p.out)[at] = lcf_from_f32<lcf_h>(x);
+    }
+}
+
 // joins the splits' parts in a fixed order and applies the epilogue.  A workgroup takes 64
 // consecutive elements: thread = (split line t / 16, four elements t % 16); 16 lines run over the
 // splits side by side and meet in LDS.
@@ -857,23 +965,27 @@ __global__ void __launch_bounds__(256) f8_join_kernel(F8Gemm p, int splits)
 
 static bool f8_is_thin(int M, int N, int K, bool wide);
 struct F8Plan {
-    int thin, big, tiles_m, tiles_n, splits, ksteps;
+    int thin, few, big, tiles_m, tiles_n, splits, ksteps;
 };
 static F8Plan f8_plan(int M, int N, int K, bool wide)
 {
     F8Plan q;
     q.thin = f8_is_thin(M, N, K, wide);
+    q.few = M <= 64 && K > 0;
     const long long t256 = (long long)((M + 255) / 256) * ((N + 255) / 256);
-    q.big = t256 >= 192;
-    const int bm = q.big ? 256 : 128;
+    const long long t128 = (long long)((M + 127) / 128) * ((N + 127) / 128);
+    // the largest tile that still gives the 256 units work: 256 x 256 (one workgroup fills a unit),
+    // 128 x 128 (two do), 64 x 128 (three do)
+    q.big = t256 >= 192 ? 2 : t128 >= 512 ? 1 : 0;
+    const int bm = q.big == 2 ? 256 : q.big == 1 ? 128 : 64, bn = q.big == 2 ? 256 : 128;
     q.tiles_m = (M + bm - 1) / bm;
-    q.tiles_n = (N + bm - 1) / bm;
+    q.tiles_n = (N + bn - 1) / bn;
     const int steps = (K + 127) / 128;
     const long long tiles = (long long)q.tiles_m * q.tiles_n;
     // a few tiles over a long sum: split it until the chip's 256 units have work, at least four
     // steps to a split
     int splits = 1;
-    if (!q.thin && tiles < 128) {
+    if (!q.thin && !q.few && tiles < 128) {
         splits = (int)(256 / tiles);
         if (splits > steps / 4) splits = steps / 4;
         if (splits < 1) splits = 1;
@@ -918,24 +1030,39 @@ template <int FA, int FB, bool WIDE, typename T> static int f8_stream_launch(con
     return LCF_OK;
 }
 
+template <int FA, int FB, bool WIDE, int WM, int WN, int MT>
+static int f8_tile_launch(const F8Gemm &p, unsigned grid, hipStream_t st)
+{
+    constexpr int room = 2 * (WM * MT * 16 + WN * 64) * 132;
+    // more LDS than a launch may take unasked
+    if (room > 65536 && hipFuncSetAttribute((const void *)f8_gemm_kernel<FA, FB, WIDE, WM, WN, MT>,
+                                            hipFuncAttributeMaxDynamicSharedMemorySize, room) != hipSuccess)
+        return LCF_ERR_LAUNCH;
+    f8_gemm_kernel<FA, FB, WIDE, WM, WN, MT><<<grid, WM * WN * 64, room, st>>>(p);
+    LCF_CHECK_LAUNCH();
+    return LCF_OK;
+}
+
 template <int FA, int FB, bool WIDE> static int f8_gemm_launch2(const F8Gemm &p, const F8Plan &q, hipStream_t st)
 {
     if (q.thin && f8_out_ok(p.out, p.ldo, p.code)) return f8_stream_launch<FA, FB, WIDE, unsigned char>(p, st);
-    const unsigned grid = (unsigned)(((long long)q.tiles_m * q.tiles_n * q.splits + 7) / 8 * 8);
-    // more LDS than a launch may take unasked
-    if (q.big) {
-        const void *f = (const void *)f8_gemm_kernel<FA, FB, WIDE, 2, 4, 8>;
-        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 512 * 132) != hipSuccess)
-            return LCF_ERR_LAUNCH;
-        f8_gemm_kernel<FA, FB, WIDE, 2, 4, 8><<<grid, 512, 2 * 512 * 132, st>>>(p);
-    } else {
-        const void *f = (const void *)f8_gemm_kernel<FA, FB, WIDE, 2, 2, 4>;
-        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * 256 * 132) != hipSuccess)
-            return LCF_ERR_LAUNCH;
-        f8_gemm_kernel<FA, FB, WIDE, 2, 2, 4><<<grid, 256, 2 * 256 * 132, st>>>(p);
+    if (q.few) {
+        // a wave for each turn along k, eight at most, 16 where there are few columns; and as many as
+        // there are pieces of 16 rows to write
+        const int turns = (p.K + 511) / 512, most = p.N >= 4096 || p.M > 16 ? 8 : 16, mt = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
+        int waves = turns < most ? turns : most;
+        if (waves < mt) waves = mt;
+        const unsigned g = (unsigned)((p.N + 15) / 16), nt = waves * 64, room = waves * mt * 1024;
+        if (mt == 1) f8_few_kernel<FA, FB, WIDE, 1><<<g, nt, room, st>>>(p);
+        else if (mt == 2) f8_few_kernel<FA, FB, WIDE, 2><<<g, nt, room, st>>>(p);
+        else f8_few_kernel<FA, FB, WIDE, 4><<<g, nt, room, st>>>(p);
+        LCF_CHECK_LAUNCH();
+        return LCF_OK;
     }
-    LCF_CHECK_LAUNCH();
-    return LCF_OK;
+    const unsigned grid = (unsigned)(((long long)q.tiles_m * q.tiles_n * q.splits + 7) / 8 * 8);
+    if (q.big == 2) return f8_tile_launch<FA, FB, WIDE, 2, 4, 8>(p, grid, st);
+    if (q.big == 1) return f8_tile_launch<FA, FB, WIDE, 2, 2, 4>(p, grid, st);
+    return f8_tile_launch<FA, FB, WIDE, 2, 2, 2>(p, grid, st);
 }
 template <int FA, int FB> static int f8_gemm_launch(const F8Gemm &p, const F8Plan &q, hipStream_t st)
 {

@@ -191,19 +191,8 @@ at::Tensor bordered(const at::Tensor &t, long long to, long long &ld)
     return out.view(t.scalar_type()).narrow(1, 0, C);
 }
 
-F8 f8_operand(PyObject *pair, const char *name)
+F8 f8_operand(const at::Tensor &data, const at::Tensor &scale, const char *name)
 {
-    PyObject *d = nullptr, *s = nullptr;
-    if (PyTuple_Check(pair) && PyTuple_GET_SIZE(pair) == 2) {
-        d = PyTuple_GET_ITEM(pair, 0);
-        s = PyTuple_GET_ITEM(pair, 1);
-    } else if (PyList_Check(pair) && PyList_GET_SIZE(pair) == 2) {
-        d = PyList_GET_ITEM(pair, 0);
-        s = PyList_GET_ITEM(pair, 1);
-    } else {
-        fail(PyExc_TypeError, std::string("f8_matmul: ") + name + " must be (data, scale)");
-    }
-    const at::Tensor &data = need(d), &scale = need(s);
     on_gpu(data);
     beside(scale, data, "f8_matmul");
     F8 m;
@@ -222,6 +211,21 @@ F8 f8_operand(PyObject *pair, const char *name)
     m.data = bordered(data, 16, m.ld);
     m.scale = bordered(scale, 4, m.lds);
     return m;
+}
+
+F8 f8_operand(PyObject *pair, const char *name)
+{
+    PyObject *d = nullptr, *s = nullptr;
+    if (PyTuple_Check(pair) && PyTuple_GET_SIZE(pair) == 2) {
+        d = PyTuple_GET_ITEM(pair, 0);
+        s = PyTuple_GET_ITEM(pair, 1);
+    } else if (PyList_Check(pair) && PyList_GET_SIZE(pair) == 2) {
+        d = PyList_GET_ITEM(pair, 0);
+        s = PyList_GET_ITEM(pair, 1);
+    } else {
+        fail(PyExc_TypeError, std::string("f8_matmul: ") + name + " must be (data, scale)");
+    }
+    return f8_operand(need(d), need(s), name);
 }
 
 // x [R, C] -> rows form, columns form, column sums [ceil(R / 128), C] (each where asked for)
@@ -318,12 +322,6 @@ at::Tensor f8_product(const at::Tensor &x, const F8 &b, const at::Tensor *scale,
     if (out.defined()) return out;
     return f8_mm(f8_quant(x, LCF_E4M3, false, true, false, false, st).rows, b, scale, shift, relu,
                  type_code(x.scalar_type()), nullptr, st);
-}
-
-F8 weight_image(const at::Tensor &w, bool transpose, int fmt, void *st)
-{
-    Quant q = f8_quant(w, fmt, true, !transpose, transpose, false, st);
-    return transpose ? q.cols : q.rows;
 }
 
 // ---- entry points
@@ -467,11 +465,14 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     }
 };
 
-Tensor f8_linear_fwd(const Tensor &x, const Tensor &w, const Tensor *bias, bool turned, const F8 *x8)
+// back: the image that the input's gradient takes, made from the same reading of the weight
+Tensor f8_linear_fwd(const Tensor &x, const Tensor &w, const Tensor *bias, bool turned, const F8 *x8, F8 *back)
 {
     const On on(x);
     beside(w, x, "f8_linear");
-    const F8 image = weight_image(w, turned, LCF_E4M3, on.st);
+    const Quant q = f8_quant(w, LCF_E4M3, true, !turned || back, turned || back, false, on.st);
+    const F8 &image = turned ? q.cols : q.rows;
+    if (back) *back = turned ? q.rows : q.cols;
     Tensor shift;
     if (bias) {
         beside(*bias, x, "f8_linear");
@@ -489,10 +490,12 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Maybe &bias, bool turned,
                           const F8 *x8)
     {
-        ctx->save_for_backward({x, w});
+        F8 back;
+        Tensor y = f8_linear_fwd(x, w, maybe(bias), turned, x8, x.requires_grad() ? &back : nullptr);
+        ctx->save_for_backward({x, w, back.data, back.scale});
         ctx->saved_data["turned"] = turned;
         ctx->saved_data["bias"] = (int64_t)(maybe(bias) ? type_code(bias->scalar_type()) : -1);
-        return f8_linear_fwd(x, w, maybe(bias), turned, x8);
+        return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
@@ -510,7 +513,7 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
         // columns form and the bias's sums come out of one reading
         F8 image;
         if (need_x) {
-            image = weight_image(w, !turned, LCF_E4M3, on.st);
+            image = f8_operand(saved[2], saved[3], "weight");
             dx = f8_fused(dy, image, nullptr, nullptr, false, on.st);
         }
         const bool rows = need_x && !dx.defined();
@@ -593,7 +596,7 @@ PyObject *py_f8_linear(PyObject *, Args a, Py_ssize_t n)
         if (at::GradMode::is_enabled() && (wants(&x) || wants(&w) || wants(bias)))
             return wrap(F8Linear::apply(x, w, bias ? Maybe(*bias) : Maybe(), turned, p8));
         at::AutoDispatchBelowADInplaceOrView below;
-        return wrap(f8_linear_fwd(x, w, bias, turned, p8));
+        return wrap(f8_linear_fwd(x, w, bias, turned, p8, nullptr));
     });
 }
 // rms_norm(x, weight, eps, residual) -> y, or (y, h) with a residual; differentiable

@@ -180,10 +180,12 @@ def test_f8_matmul_epilogue_and_out(cuda):
         assert bool((room[:, :20] == 7).all()) and bool((room[:, 20 + N:] == 7).all())
 
 
-def test_f8_matmul_split_sum_is_repeatable_and_joined(cuda):
-    M, N, K = 40, 64, 70000
+@pytest.mark.parametrize("M", [40, 100])
+def test_f8_matmul_split_sum_is_repeatable_and_joined(cuda, M):
+    """A long sum split over the waves of a workgroup (few rows) and over workgroups (a workspace)."""
+    N, K = 64, 70000
     a, b = _rows(10, M, K), _rows(11, N, K)
-    assert ops._lib.lib().lcf_f8_gemm_workspace_bytes(M, N, K, 0) > 0
+    assert (ops._lib.lib().lcf_f8_gemm_workspace_bytes(M, N, K, 0) > 0) == (M > 64)
     xa, xb = ops.f8_rows(a.to(cuda)), ops.f8_rows(b.to(cuda))
     qa, qb = ref.value(*ref.quantise(a)), ref.value(*ref.quantise(b))
     bias = torch.randn((N,), generator=_gen(12)).to(cuda)
@@ -523,7 +525,7 @@ def test_on_another_stream_and_captured(cuda):
     M, C, D = 200, 128, 64
     x, r = _rows(90, M, C).to(cuda), _rows(91, M, C).to(cuda)
     w8 = ops.f8_weight_image(_rows(92, D, C, size=0.1).to(cuda))
-    big = ops.f8_rows(_rows(93, 16, 40000).to(cuda))
+    big = ops.f8_rows(_rows(93, 100, 40000).to(cuda))
     grads = [t.to(cuda) for t in _grads(94, [torch.float32], 20)]
 
     def run():

@@ -122,7 +122,8 @@ def test_abi_refuses_bad_8_bit_operands():
                              n, None)
     for bad in (dict(a=None), dict(lda=60), dict(lda=48), dict(a=4097), dict(sa=None), dict(ldsa=1), dict(af=2),
                 dict(b=None), dict(ldb=63), dict(sb=4097), dict(bf=5), dict(M=-1), dict(K=-1), dict(out=None),
-                dict(ldo=3), dict(od=3), dict(K=70000, lda=70016, ldb=70016, ldsa=548, ldsb=548)):
+                dict(ldo=3), dict(od=3), dict(M=100, K=70000, lda=70016, ldb=70016, ldsa=548, ldsb=548)):
         assert gemm(**bad) == ARG, bad
-    assert gemm(K=70000, lda=70016, ldb=70016, ldsa=548, ldsb=548, ws=4096, n=16) == WORKSPACE
+    assert gemm(M=100, K=70000, lda=70016, ldb=70016, ldsa=548, ldsb=548, ws=4096, n=16) == WORKSPACE
+    assert gemm(lda=1 << 23) == UNSUPPORTED and gemm(ldb=1 << 23) == UNSUPPORTED
     assert gemm(M=0, a=None) == 0 and gemm(N=0, b=None) == 0
