@@ -749,6 +749,7 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  * q[r][c] * 2^(s[r / 128][c / 128] - 127).  2^e is the smallest power of two that brings the
  * block's largest finite magnitude inside the format (448 for e4m3, 57344 for e5m2), e >= -126;
  * a block of zeros has e = 0; infinities and NaN are stored as NaN and do not enter the scale.
+ * (Scale bytes are 1 to 254: 0 and 255 have no meaning here.)
  * quant: x [R, C] (ldx elements between rows) ->
  *   rows form (q / s, NULL = not wanted), blocks of 1 x 128 along each row, and / or
  *   columns form (qt / st, NULL = not wanted): the rows form of x^T, [C, R], blocks of 128 along

@@ -258,7 +258,8 @@ _lib = None
 
 
 def build(force=False):
-    """Compile liblcf.so in-tree with hipcc for gfx950 (cross-compiles without a GPU)."""
+    """Compile liblcf.so in-tree with hipcc for gfx950 (cross-compiles without a GPU), the GPU-free
+    twin and the row operators' host module."""
     if force:
         subprocess.check_call(["make", "-s", "-C", os.path.join(_HERE, "csrc"), "clean"])
     subprocess.check_call(["make", "-s", "-j4", "-C", os.path.join(_HERE, "csrc")])

@@ -13,11 +13,6 @@ typedef float lcf_f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short lcf_s8u __attribute__((ext_vector_type(8), aligned(2)));
 typedef unsigned lcf_u2u __attribute__((ext_vector_type(2), aligned(4)));
 
-template <typename T> struct LcfType;
-template <> struct LcfType<float> { static constexpr int code = LCF_F32; };
-template <> struct LcfType<lcf_b> { static constexpr int code = LCF_BF16; };
-template <> struct LcfType<lcf_h> { static constexpr int code = LCF_F16; };
-
 static inline int lcf_type_size(int code) { return code == LCF_F32 ? 4 : 2; }
 static inline bool lcf_is_type(int code) { return code == LCF_F32 || code == LCF_BF16 || code == LCF_F16; }
 

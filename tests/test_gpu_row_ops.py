@@ -224,7 +224,8 @@ def test_f8_matmul_ignores_what_lies_behind_the_last_column(cuda):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", [(1, 16, 16), (50, 64, 256), (700, 256, 64), (300, 100, 37), (129, 1, 130)])
+@pytest.mark.parametrize("shape", [(1, 16, 16), (50, 64, 256), (700, 256, 64), (300, 100, 37), (129, 1, 130),
+                                   (4500, 256, 64), (4099, 64, 200), (4200, 300, 520)])
 def test_f8_linear_forward_and_gradients(cuda, shape, dtype):
     M, N, K = shape
     x = _rows(17, M, K, dtype).to(cuda).requires_grad_(True)
@@ -560,3 +561,94 @@ def test_on_another_stream_and_captured(cuda):
         torch.cuda.synchronize()
         for g, out in graphs:
             assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_empty_rows_broadcast_gradients_and_unused_outputs(cuda):
+    """Gradients as autograd hands them over: expanded (a sum's), missing (an output nobody used), of
+    rows that are a view; a weight that needs none."""
+    x, r = _rows(100, 6, 40).to(cuda), _rows(101, 6, 40).to(cuda)
+    w = (1.0 + 0.1 * torch.randn((40,), generator=_gen(102))).to(cuda)
+    for use_y, use_h in ((True, False), (False, True), (True, True)):
+        a, b, c = (t.clone().requires_grad_(True) for t in (x, r, w))
+        y, h = ops.rms_norm(a, c, 1e-6, b)
+        loss = (y.sum() if use_y else 0.0) + (3.0 * h.sum() if use_h else 0.0)
+        loss.backward()
+        _, hh, inv = ref.rms_norm(x, w, 1e-6, r)
+        want = torch.zeros((6, 40), dtype=torch.float64)
+        if use_y:
+            dy = torch.ones((6, 40))
+            want, want_w = ref.rms_norm_bwd(hh, w, inv, dy)
+            _within(c.grad, want_w, 300 * F32 * (hh * inv).abs().sum(0))
+            size = inv * (w.double().cpu().abs() + hh.abs() * inv ** 2
+                          * (w.double().cpu() * hh).abs().mean(1, keepdim=True))
+        else:
+            assert c.grad is None or bool((c.grad == 0).all())
+            size = torch.zeros_like(want)
+        if use_h:
+            want = want + 3.0
+        _within(a.grad, want, 3 * _chain(40) * F32 * (size + 3.0))
+        assert torch.equal(a.grad, b.grad)
+    # one row of x shared by all rows, and a residual that is a view
+    row = _rows(103, 1, 40).to(cuda).requires_grad_(True)
+    y, h = ops.rms_norm(row.expand(6, 40), w, 1e-6, _rows(104, 6, 80).to(cuda)[:, 40:])
+    (g,) = torch.autograd.grad(y.sum() + h.sum(), (row,))
+    wide = row.detach().expand(6, 40).contiguous().requires_grad_(True)
+    y, h = ops.rms_norm(wide, w, 1e-6, _rows(104, 6, 80).to(cuda)[:, 40:])
+    (gw,) = torch.autograd.grad(y.sum() + h.sum(), (wide,))
+    assert torch.equal(g, gw.sum(0, keepdim=True))
+    # products of nothing
+    e = torch.zeros((0, 16), device=cuda, requires_grad=True)
+    m = _rows(105, 8, 16).to(cuda).requires_grad_(True)
+    bias = torch.zeros((8,), device=cuda, requires_grad=True)
+    ge, gm, gb = torch.autograd.grad(ops.f8_linear(e, m, bias).sum(), (e, m, bias))
+    assert ge.shape == (0, 16) and bool((gm == 0).all()) and bool((gb == 0).all())
+    # leading dimensions, a weight stored [K, N], rows in 8-bit form already, no gradient asked for
+    t = _rows(106, 30, 16).to(cuda)
+    want = ops.f8_linear(t, m.detach())
+    assert torch.equal(ops.f8_linear(t.view(5, 6, 16), m.detach()).view(30, 8), want)
+    assert torch.equal(ops.f8_linear(t, m.detach().t().contiguous(), turned=True), want)
+    assert torch.equal(ops.f8_linear(t, m.detach(), x8=ops.f8_rows(t)), want)
+    with torch.no_grad():
+        assert torch.equal(ops.f8_linear(t, m), want)
+
+
+def test_f8_matmul_into_outputs_that_start_anywhere(cuda):
+    """Odd columns of a wider matrix, for few rows, tiles and thin layers over many rows."""
+    for M, N, K in ((5, 40, 300), (300, 264, 200), (4100, 64, 96), (4100, 256, 512)):
+        a, b = ops.f8_rows(_rows(110, M, K).to(cuda)), ops.f8_weight_image(_rows(111, N, K).to(cuda))
+        for dtype in DTYPES:
+            want = ops.f8_matmul(a, b, out_dtype=dtype)
+            room = torch.full((M, N + 9), 5.0, dtype=dtype, device=cuda)
+            ops.f8_matmul(a, b, out=room[:, 3:3 + N])
+            assert torch.equal(room[:, 3:3 + N], want)
+            assert bool((room[:, :3] == 5).all()) and bool((room[:, 3 + N:] == 5).all())
+
+
+def test_operators_past_32_bit_offsets(cuda):
+    """Rows whose bytes and elements lie beyond 2^32 and 2^31: the last ones are what they are alone."""
+    R, C = 140000, 16384
+    x = torch.zeros((R, C), dtype=torch.bfloat16, device=cuda)
+    tail = _rows(120, 70, C, torch.bfloat16).to(cuda)
+    x[-70:] = tail
+    w = ops.f8_weight_image(_rows(121, 16, C, size=C ** -0.5).to(cuda))
+    y = ops.rms_norm(x, None, 1e-6)
+    assert torch.equal(y[-70:], ops.rms_norm(tail, None, 1e-6)) and float(y[:1000].abs().sum()) == 0
+    del y
+    q = ops.f8_rows(x)
+    alone = ops.f8_rows(tail)
+    assert torch.equal(q.data[-70:].view(torch.uint8), alone.data.view(torch.uint8))
+    got = ops.f8_matmul(q, w)
+    # the two calls may add the same exact products in another order: each is within the bound of one sum
+    qa, qb = (ref.value(v.data.cpu(), v.scale.cpu().view(torch.uint8).int() - 127, h) for v, h in ((alone, 1), (w, 128)))
+    want = qa @ qb.t()
+    _within(got[-70:], want, _product_bound(qa, qb, C, want, torch.float32))
+    _within(ops.f8_matmul(alone, w), want, _product_bound(qa, qb, C, want, torch.float32))
+    assert float(got[:1000].abs().sum()) == 0
+    del q, got
+    xt = ops.f8_cols(x)
+    assert torch.equal(xt.data[:, -70:].float(), ops.f8_cols(x[-(R % 128 or 128):]).data[:, -70:].float())
+    del xt
+    total = ops.clip_norm_([x], 1.0)
+    want, (part,) = ref.clip([tail], 1.0)
+    _within(total, want, 2 * F32 * want)
+    _within(x[-70:], part, (half_step(torch.bfloat16) + 6 * F32) * part.abs() * 1.001 + tiny(torch.bfloat16))
