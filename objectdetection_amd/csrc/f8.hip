@@ -763,6 +763,8 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
         const int left = p.M - m0 < 16 ? (int)(p.M - m0) : 16;
         const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
             (char *)p.out + m0 * p.ldo * EO, 0, ((left - 1) * (int)p.ldo + p.N) * EO, 0x00020000);
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        u4 o[16 / W];
 #pragma unroll
         for (int q = 0; q < 16 / W; ++q) {
             const int n = n0 + (WIDE ? 16 * q + 4 * g : 32 * q + 8 * g);
@@ -781,27 +783,45 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
 #pragma unroll
                 for (int i = 0; i < W; ++i) v[i] = v[i] < 0.f ? 0.f : v[i]; // NaN stays
             }
-            typedef unsigned u4 __attribute__((ext_vector_type(4)));
-            u4 o;
             if constexpr (WIDE) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = __float_as_uint(v[i]);
+                for (int i = 0; i < 4; ++i) o[q][i] = __float_as_uint(v[i]);
             } else if (p.code == LCF_BF16) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    o[i] = __builtin_bit_cast(unsigned short, lcf_from_f32<lcf_b>(v[2 * i])) |
-                           (unsigned)__builtin_bit_cast(unsigned short, lcf_from_f32<lcf_b>(v[2 * i + 1])) << 16;
+                    o[q][i] = __builtin_bit_cast(unsigned short, lcf_from_f32<lcf_b>(v[2 * i])) |
+                              (unsigned)__builtin_bit_cast(unsigned short, lcf_from_f32<lcf_b>(v[2 * i + 1])) << 16;
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    o[i] = __builtin_bit_cast(unsigned short, lcf_from_f32<lcf_h>(v[2 * i])) |
-                           (unsigned)__builtin_bit_cast(unsigned short, lcf_from_f32<lcf_h>(v[2 * i + 1])) << 16;
+                    o[q][i] = __builtin_bit_cast(unsigned short, lcf_from_f32<lcf_h>(v[2 * i])) |
+                              (unsigned)__builtin_bit_cast(unsigned short, lcf_from_f32<lcf_h>(v[2 * i + 1])) << 16;
             }
-            // N is a multiple of W: a piece is inside or outside as a whole.  Stored past the caches (nt):
-            // the output is as large as they are (a training step's three products over 136000 rows of
-            // 64 and 256 columns: 125 -> 121 us; the same for the rows' loads made it 143)
-            const int at = n < p.N && r16 < left ? (r16 * (int)p.ldo + n) * EO : (int)0x80000000;
-            __builtin_amdgcn_raw_buffer_store_b128(o, to, at, 0, 2);
+        }
+        // Two pieces of a row are one 128-byte line, and a row's four lanes would store half of it at a
+        // time (1.3 times the bytes then reached memory).  Lanes eight apart trade a piece, so that eight
+        // lanes store whole lines of eight rows.  N is a multiple of W: a piece is inside or outside as a
+        // whole.  Stored past the caches (nt): the output is as large as they are (a training step's three
+        // products over 136000 rows of 64 and 256 columns: 125 -> 121 us; the same for the rows' loads
+        // made it 143).
+        const bool low = r16 < 8;
+        const int row = r16 & 7;
+#pragma unroll
+        for (int q = 0; q < 16 / W; q += 2) {
+            u4 first, second;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned mine = low ? o[q][i] : o[q + 1][i];
+                const unsigned got = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(low ? o[q + 1][i] : o[q][i]), 0x128,
+                                                                           0xF, 0xF, false);
+                first[i] = low ? mine : got;
+                second[i] = low ? got : mine;
+            }
+            const int n = n0 + (WIDE ? 16 * (q + !low) + 4 * g : 32 * (q + !low) + 8 * g);
+            const int at = (row * (int)p.ldo + n) * EO;
+            __builtin_amdgcn_raw_buffer_store_b128(first, to, n < p.N && row < left ? at : (int)0x80000000, 0, 2);
+            __builtin_amdgcn_raw_buffer_store_b128(
+                second, to, n < p.N && row + 8 < left ? at + 8 * (int)p.ldo * EO : (int)0x80000000, 0, 2);
         }
     };
     // everything asked for so far is here: the loop's waits then count its own operations only
