@@ -9,6 +9,9 @@
 // fp32); LPR lanes share a row, so a wave works on 64 / LPR narrow rows at once, and 16 lanes hold
 // exactly one 128-column scale block of the 8-bit form: its largest magnitude is four lane swaps.
 // Rows wider than a wave's registers take a workgroup (LPR = 256 or 1024).
+// Measured with residual: 16384 x 4096 bf16 forward 95 us (5.6 TB/s), backward 109 us (4.9 TB/s) and
+// 8 us for the weight's gradient; 136000 x 64 fp32 28 + 25 + 4 us; 40000 x 256 bf16 to 8-bit rows 16 us
+// (4.5 TB/s); one row of 4096 3.5 us, the smallest kernel's duration.
 #include "rows.h"
 
 #define RN_MAX_WIDTH 16384
