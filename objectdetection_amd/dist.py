@@ -125,8 +125,10 @@ class FlatGradAllReduce:
         is copied into the buffer -- one reading and one writing of the buffer less."""
         params = self.params
         views = [v for vs in self.views for v in vs]
+        kinds = (torch.float32, torch.bfloat16, torch.float16)
         if self.attach or not self.flat.is_cuda or any(
-                p.grad is None or p.grad is v or p.grad.stride() != v.stride()
+                p.grad is None or p.grad is v or p.grad.layout != torch.strided
+                or p.grad.stride() != v.stride() or p.grad.dtype not in kinds
                 for p, v in zip(params, views)):
             self.collect()
             return self.clip_norm_(max_norm)
