@@ -165,7 +165,8 @@ class SparseConvolution(SparseModule):
     def _pointwise_f8(self, x, w, scale, shift, relu, f8):
         """Rows x [K, Cin] (or, in inference, their 8-bit form ``f8`` already) through w [Cin, Cout]
         on 8-bit operands."""
-        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad):
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or (
+                self.bias is not None and self.bias.requires_grad)):
             out = ops.f8_linear(x, w, self.bias, turned=True)
             return torch.relu(out) if relu else out
         if self.bias is not None:

@@ -76,6 +76,13 @@ def test_pointwise_conv_in_8_bit_form_trains(cuda, dtype):
     _near(feats.grad, _q(g) @ _q(w, 128).t(), share)
     _near(conv.weight.grad.view(256, 64), _q(feats.detach().t()) @ _q(g.t()).t(), 1e-5)
     _near(conv.bias.grad, g.double().sum(0), 1e-5)
+    # a bias that alone wants a gradient gets one
+    conv.weight.requires_grad_(False)
+    conv.bias.grad = None
+    x.features = feats.detach()
+    with ops.conv_math("f8"):
+        conv(x).features.backward(g.to(cuda))
+    _near(conv.bias.grad, g.double().sum(0), 1e-5)
     plain = conv(x).features  # the default mode is what it was
     assert torch.equal(plain, torch.mm(feats, w.to(dtype)) + conv.bias.to(dtype))
 
