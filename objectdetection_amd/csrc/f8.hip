@@ -9,9 +9,9 @@
 //     and takes one E8M0 scale byte per row and 32 columns of either operand: with scale blocks of
 //     128 along k one instruction covers exactly one block of both operands, and the scales cost no
 //     vector work.  The instruction adds its products in groups of eight along k and keeps 13 bits
-//     below the largest of a group (measured; between groups it adds in fp32): an error of up to
-//     2^-10 of a group's sum of magnitudes, 1.5e-5 of the result on random data -- below a 16-bit
-//     store's half step (2^-9 bf16, 2^-12 fp16), but not what an fp32 output promises.
+//     below the largest of a group (measured; between groups it adds in fp32): an error of at most
+//     2^-10 of a group's sum of magnitudes, and 1.5e-5 of the result on random data -- a 16-bit store
+//     rounds by up to 2^-8 (bf16) or 2^-11 (fp16) of it.  Not what an fp32 output promises.
 //   fp32 outputs: the bytes become bf16 in registers, scaled (v_cvt_scalef32_pk_bf16_*: q 2^e is
 //     exact), and v_mfma_f32_16x16x32_bf16 adds the exact products in fp32, at half the peak rate.
 #include "rows.h"

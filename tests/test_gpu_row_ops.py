@@ -195,6 +195,23 @@ def test_f8_matmul_split_sum_is_repeatable_and_joined(cuda, M):
     assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(100, 64, 9000), (100, 300, 6000), (70, 20, 5005), (300, 40, 4100)])
+def test_f8_matmul_split_sums_of_every_type(cuda, shape, dtype):
+    M, N, K = shape
+    assert ops._lib.lib().lcf_f8_gemm_workspace_bytes(M, N, K, ops._TYPE_CODE[dtype]) > 0
+    a, b = _rows(13, M, K), _rows(14, N, K, size=K ** -0.5)
+    scale, shift = torch.rand((N,), generator=_gen(15)) + 0.5, torch.randn((N,), generator=_gen(16))
+    qa, qb = ref.value(*ref.quantise(a)), ref.value(*ref.quantise(b, h=128), 128)
+    y = qa @ qb.t()
+    got = ops.f8_matmul(ops.f8_rows(a.to(cuda)), ops.f8_weight_image(b.to(cuda)), scale.to(cuda), shift.to(cuda), True,
+                        dtype)
+    want = (y * scale.double() + shift.double()).clamp(min=0)
+    bound = scale.double() * _product_bound(qa, qb, K, y, torch.float32 if dtype == torch.float32 else dtype)
+    _within(got, want, bound + 4 * F32 * (y.abs() * scale.double() + shift.double().abs())
+            + half_step(dtype) * want * 1.01 + tiny(dtype))
+
+
 def test_f8_matmul_empty_sizes(cuda):
     a = ops.f8_rows(torch.zeros((0, 40), device=cuda))
     b = ops.f8_weight_image(_rows(13, 8, 40).to(cuda))
@@ -529,13 +546,17 @@ def test_on_another_stream_and_captured(cuda):
     big = ops.f8_rows(_rows(93, 100, 40000).to(cuda))
     grads = [t.to(cuda) for t in _grads(94, [torch.float32], 20)]
 
+    wide = ops.f8_rows(_rows(95, 3600, 256).to(cuda))
+
     def run():
         a8, h = ops.rms_norm_f8(x, None, 1e-6, r)
         y = ops.f8_matmul(a8, w8)
         z = ops.f8_matmul(big, big)  # a split sum: uses a workspace
+        t = ops.f8_matmul(wide, wide, out_dtype=torch.bfloat16)  # 256 x 256 tiles
+        u = ops.f8_matmul(wide, wide)
         flat = torch.empty((sum(g.numel() for g in grads),), device=cuda)
         total = ops.clip_norm_(grads, 1.0, out=flat)
-        return h, y, z, flat, total
+        return h, y, z, t, u, flat, total
     want = [t.clone() for t in run()]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -543,6 +564,7 @@ def test_on_another_stream_and_captured(cuda):
         got = run()
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(run(), want))
     graphs = []
     for _ in range(2):
         g = torch.cuda.CUDAGraph()
