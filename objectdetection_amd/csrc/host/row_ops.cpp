@@ -584,6 +584,8 @@ PyObject *py_f8_linear(PyObject *, Args a, Py_ssize_t n)
             x.size(1) != w.size(turned ? 0 : 1))
             fail(PyExc_ValueError, "f8_linear: x " + shape(x) + " against weight " + shape(w) +
                                        " (float32, bfloat16 or float16)");
+        if (at::GradMode::is_enabled() && wants(&w) && x.size(0) > 1 << 22)
+            fail(PyExc_ValueError, "f8_linear: at most 2^22 rows where the weight wants a gradient (its product sums over them)");
         const long long out = w.size(turned ? 1 : 0);
         if (bias && (bias->dim() != 1 || bias->size(0) != out || type_code(bias->scalar_type()) < 0))
             fail(PyExc_ValueError, "f8_linear: bias must have " + std::to_string(out) + " float elements");

@@ -1373,6 +1373,7 @@ def f8_linear(x, weight, bias=None, turned=False, x8=None):
     operands: -> [..., N] of x's type, differentiable in all three (weight and bias keep their own
     types): y, dx = dy W and dW = dy^T x are products of 8-bit operands whose scale blocks lie along
     the axis that the product sums over; the rounding is passed through unchanged.  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.
+    At most 2^22 rows where the weight wants a gradient.
     Error of an operand: half a step of e4m3, 2^-4 of a value, plus 2^-10 of its block's scale for
     small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
     if x.dim() == 2:
