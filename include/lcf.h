@@ -758,7 +758,8 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  *   sums != NULL: the columns' sums over each 128 rows, [ceil(R / 128), C] fp32, for lcf_sum_parts
  *   (a bias gradient out of the same reading; q and qt may then both be NULL).
  *   Bytes between the last column and the next multiple of 16, and scale bytes between the last
- *   block and the next multiple of 4, are written as zeros.
+ *   block and the next multiple of 4, are written as zeros.  C <= 2^31 - 256, and R <= 65535 * 128
+ *   where more than the rows form is asked for (LCF_ERR_UNSUPPORTED).
  * gemm: out[m][n] = act((sum_k a[m][k] b[n][k]) * scale[n] + shift[n]), a [M, K], b [N, K] in rows
  *   form, b_square != 0: b has 128 x 128 scale blocks; scale / shift fp32 or NULL, relu != 0 clamps
  *   at 0; out [M, N] of out_dtype, ldo elements between rows.  What lies in a row behind column K
@@ -766,13 +767,16 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  *   registers); bf16 / fp16: the 8-bit matrix instructions, whose sums of eight neighbouring
  *   products keep 13 bits below the largest of them (an error of at most 2^-10 of the sum of
  *   magnitudes; about 1.5e-5 of the result on random data), then one rounding.
- *   K == 0 gives act(shift).  lda, ldb <= 2^22 (LCF_ERR_UNSUPPORTED).  ws: lcf_f8_gemm_workspace_bytes(M, N, K, out_dtype) (0 for most sizes: the sum
- *   is split over workgroups only where the output has few tiles; the parts are joined in a fixed
- *   order, so results are run-to-run identical). */
+ *   K == 0 gives act(shift).  LCF_ERR_UNSUPPORTED: lda or ldb > 2^22, M or N > 2^31 - 256, N > 2^25
+ *   where M <= 64, 2^23 tiles of the output or more (the smallest are of 64 x 128 and 128 x 64).
+ *   ws: lcf_f8_gemm_workspace_bytes(M, N, K, out_dtype) (0 for most sizes: the sum is split over
+ *   workgroups only where the output has few tiles; the parts are joined in a fixed order, so
+ *   results are run-to-run identical). */
 int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtype, int fmt, int square, void *q,
                  long long ldq, unsigned char *s, int lds, void *qt, long long ldqt,
                  unsigned char *st, int ldst, float *sums, void *stream);
-/* out [n] of `dtype` = the column sums of parts [count, n], in 64 bits and a fixed order. */
+/* out [n] of `dtype` = the column sums of parts [count, n], in 64 bits and a fixed order; n <= 2^25
+ * (LCF_ERR_UNSUPPORTED). */
 int lcf_sum_parts(const float *parts, int count, int n, void *out, int dtype, void *stream);
 size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype);
 int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa, int ldsa, int a_fmt,

@@ -222,6 +222,8 @@ template <typename T> static void f8_quant_launch(const F8Quant &p, hipStream_t 
     }
 }
 
+#define F8_MOST 0x7FFFFF00 // rows or columns: the last tile's end is an int too
+
 static bool f8_form_ok(const void *q, long long ld, const unsigned char *s, int lds, int C)
 {
     return q && s && !((uintptr_t)q & 15) && !((uintptr_t)s & 3) && !(ld & 15) && !(lds & 3) && ld >= C &&
@@ -237,8 +239,9 @@ extern "C" int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtyp
     if (!x || ldx < C || (!q && !qt && !sums)) return LCF_ERR_ARG;
     if (q && !f8_form_ok(q, ldq, s, lds, C)) return LCF_ERR_ARG;
     if (qt && !f8_form_ok(qt, ldqt, st, ldst, R)) return LCF_ERR_ARG;
-    // the grid's second dimension counts 128-row tiles
-    if ((qt || square || sums) && (R + 127) / 128 > 65535) return LCF_ERR_UNSUPPORTED;
+    // columns are counted in 32 bits up to the end of a block, and the grid's second dimension counts
+    // 128-row tiles
+    if (C > F8_MOST || ((qt || square || sums) && R > 65535 * 128)) return LCF_ERR_UNSUPPORTED;
     F8Quant p{x, (unsigned char *)q, s, (unsigned char *)qt, st, sums, ldx, ldq, ldqt, R, C, lds, ldst, fmt, square};
     if (dtype == LCF_F32) f8_quant_launch<float>(p, (hipStream_t)stream);
     else if (dtype == LCF_BF16) f8_quant_launch<lcf_b>(p, (hipStream_t)stream);
@@ -1028,7 +1031,7 @@ static F8Plan f8_plan(int M, int N, int K, bool wide)
 
 extern "C" size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype)
 {
-    if (M < 1 || N < 1 || K < 1) return 0;
+    if (M < 1 || N < 1 || K < 1 || M > F8_MOST || N > F8_MOST || K > F8_MOST) return 0;
     const F8Plan q = f8_plan(M, N, K, out_dtype == LCF_F32);
     return q.splits > 1 ? (size_t)q.splits * M * N * sizeof(float) : 0;
 }
@@ -1152,9 +1155,12 @@ extern "C" int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa
     if (M == 0 || N == 0) return LCF_OK;
     if (!out || ldo < N) return LCF_ERR_ARG;
     if (K > 0 && (!f8_form_ok(a, lda, sa, ldsa, K) || !f8_form_ok(b, ldb, sb, ldsb, K))) return LCF_ERR_ARG;
+    // a tile's rows are addressed in 32 bits, and a launch has fewer than 2^32 threads (512 a tile at
+    // most, 1024 for 16 columns of a few rows)
+    if (lda > (1 << 22) || ldb > (1 << 22) || M > F8_MOST || N > F8_MOST) return LCF_ERR_UNSUPPORTED;
     const F8Plan q = f8_plan(M, N, K, out_dtype == LCF_F32);
-    // tiles are counted, and a tile's rows addressed, in 32 bits
-    if ((long long)q.tiles_m * q.tiles_n * q.splits > 0x7FFFFF00ll || lda > (1 << 22) || ldb > (1 << 22))
+    const bool thin = q.thin && f8_out_ok(out, ldo, out_dtype);
+    if (!thin && (q.few ? N > 1 << 25 : (long long)q.tiles_m * q.tiles_n * q.splits > (1 << 23) - 8))
         return LCF_ERR_UNSUPPORTED;
     if (q.splits > 1) {
         if (!ws) return LCF_ERR_ARG;

@@ -370,6 +370,7 @@ extern "C" int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, lo
 extern "C" int lcf_sum_parts(const float *parts, int count, int n, void *out, int dtype, void *stream)
 {
     if (count < 0 || n < 0 || !lcf_is_type(dtype)) return LCF_ERR_ARG;
+    if (n > 1 << 25) return LCF_ERR_UNSUPPORTED; // a launch has fewer than 2^32 threads
     if (n == 0) return LCF_OK;
     if ((count > 0 && !parts) || !out) return LCF_ERR_ARG;
     rn_dweight_kernel<<<(n + 15) / 16, 1024, 0, (hipStream_t)stream>>>(parts, count, n, out, dtype);

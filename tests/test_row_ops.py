@@ -115,6 +115,9 @@ def test_abi_refuses_bad_8_bit_operands():
         assert quant(**bad) == ARG, bad
     assert quant(R=0, x=None) == 0 and quant(C=0, x=None) == 0
     assert quant(R=1 << 30, sq=1) == UNSUPPORTED
+    last = (1 << 31) - 1  # the end of its last block is past 32 bits
+    assert quant(C=last, ldx=last, ldq=1 << 31, lds=1 << 24) == UNSUPPORTED
+    assert L.lcf_sum_parts(4096, 1, last, 8192, 0, None) == UNSUPPORTED
 
     def gemm(a=4096, lda=64, sa=4096, ldsa=4, af=0, b=4096, ldb=64, sb=4096, ldsb=4, bf=0, sq=0, M=4, N=4, K=64,
              out=8192, ldo=4, od=0, ws=None, n=0):
@@ -126,4 +129,8 @@ def test_abi_refuses_bad_8_bit_operands():
         assert gemm(**bad) == ARG, bad
     assert gemm(M=100, K=70000, lda=70016, ldb=70016, ldsa=548, ldsb=548, ws=4096, n=16) == WORKSPACE
     assert gemm(lda=1 << 23) == UNSUPPORTED and gemm(ldb=1 << 23) == UNSUPPORTED
+    for big in (dict(M=last), dict(N=last, ldo=last), dict(M=100, N=last, ldo=last), dict(N=(1 << 25) + 1, ldo=1 << 26),
+                dict(M=1 << 30, N=5, ldo=5), dict(M=1 << 20, N=1 << 20, ldo=1 << 20)):
+        assert gemm(**big) == UNSUPPORTED, big
+    assert L.lcf_f8_gemm_workspace_bytes(last, last, 64, 0) == 0
     assert gemm(M=0, a=None) == 0 and gemm(N=0, b=None) == 0
