@@ -145,6 +145,8 @@ int count(long long n, const char *who)
     if (n >= 1ll << 31) fail(PyExc_ValueError, std::string(who) + ": fewer than 2^31 rows and columns");
     return (int)n;
 }
+// a kernel is about to write t: what has saved it for a backward pass, or keeps a form of it, can tell
+void written(const at::Tensor &t) { t.unsafeGetTensorImpl()->bump_version(); }
 at::Tensor bytes(size_t n, const at::Tensor &like) { return at::empty({(int64_t)(n < 256 ? 256 : n)}, like.options().dtype(at::kByte)); }
 
 // ---- 8-bit form
@@ -288,6 +290,7 @@ at::Tensor f8_mm(const F8 &a, const F8 &b, const at::Tensor *scale, const at::Te
     const size_t n = L.f8_gemm_workspace_bytes(M, N, K, code);
     at::Tensor ws;
     if (n) ws = bytes(n, a.data);
+    if (to) written(out);
     check(L.f8_gemm(K ? a.q() : nullptr, a.ld, K ? a.s() : nullptr, (int)a.lds, a.fmt, K ? b.q() : nullptr, b.ld,
                     K ? b.s() : nullptr, (int)b.lds, b.fmt, b.square, M, N, K, ptr(scale), ptr(shift), relu,
                     out.data_ptr(), M > 1 ? (long long)out.stride(0) : N, code, n ? ws.data_ptr() : nullptr,
@@ -378,6 +381,13 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using Maybe = std::optional<Tensor>;
 const Tensor *maybe(const Maybe &t) { return t && t->defined() ? &*t : nullptr; }
+// the gradients are kernels' outputs, with no graph of their own: one made for a second derivative
+// (create_graph) would leave their share out without a word
+void once(const char *who)
+{
+    if (at::GradMode::is_enabled())
+        fail(PyExc_RuntimeError, std::string(who) + " is differentiable once: no backward pass with create_graph=True");
+}
 bool wants(const Tensor *t) { return t && t->requires_grad(); }
 
 struct Normed {
@@ -435,6 +445,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        once("rms_norm");
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list saved = ctx->get_saved_variables();
         const bool two = ctx->saved_data["two"].toBool();
@@ -499,6 +510,7 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        once("f8_linear");
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1];
@@ -584,9 +596,10 @@ PyObject *py_f8_linear(PyObject *, Args a, Py_ssize_t n)
             x.size(1) != w.size(turned ? 0 : 1))
             fail(PyExc_ValueError, "f8_linear: x " + shape(x) + " against weight " + shape(w) +
                                        " (float32, bfloat16 or float16)");
-        if (at::GradMode::is_enabled() && wants(&w) && x.size(0) > 1 << 22)
-            fail(PyExc_ValueError, "f8_linear: at most 2^22 rows where the weight wants a gradient (its product sums over them)");
+        if (at::GradMode::is_enabled() && (wants(&w) || wants(bias)) && x.size(0) > 1 << 22)
+            fail(PyExc_ValueError, "f8_linear: at most 2^22 rows where weight or bias wants a gradient (a sum over them)");
         const long long out = w.size(turned ? 1 : 0);
+        if (x.size(1) > 1 << 22 || out > 1 << 22) fail(PyExc_ValueError, "f8_linear: at most 2^22 columns");
         if (bias && (bias->dim() != 1 || bias->size(0) != out || type_code(bias->scalar_type()) < 0))
             fail(PyExc_ValueError, "f8_linear: bias must have " + std::to_string(out) + " float elements");
         F8 x8;
@@ -667,12 +680,16 @@ PyObject *py_clip(PyObject *, Args a, Py_ssize_t n)
                     fail(PyExc_ValueError, "out must be tensors of the gradients' sizes and strides");
                 e.out = o.data_ptr();
                 e.out_dtype = type_code(o.scalar_type());
+                written(o);
+            } else if (clip && !flat) {
+                written(g);
             }
         }
         if (flat) {
             const at::Tensor &o = take(a[1], "out");
             if (!o.is_contiguous() || o.numel() != total)
                 fail(PyExc_ValueError, "out must be a contiguous tensor with as many elements as the gradients have together");
+            written(o);
             char *at = (char *)o.data_ptr();
             for (lcf_grad &e : t) {
                 e.out = at;

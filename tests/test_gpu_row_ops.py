@@ -674,3 +674,40 @@ def test_operators_past_32_bit_offsets(cuda):
     want, (part,) = ref.clip([tail], 1.0)
     _within(total, want, 2 * F32 * want)
     _within(x[-70:], part, (half_step(torch.bfloat16) + 6 * F32) * part.abs() * 1.001 + tiny(torch.bfloat16))
+
+
+def test_second_derivatives_and_too_many_rows_are_refused(cuda):
+    x, w = _rows(120, 6, 16).to(cuda).requires_grad_(), _rows(121, 8, 16).to(cuda).requires_grad_()
+    for y in (ops.rms_norm(x), ops.f8_linear(x, w)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+    many = torch.zeros((1, 16), device=cuda).expand((1 << 22) + 1, 16)  # 2^22 + 1 rows in 64 bytes
+    bias = torch.zeros((8,), device=cuda, requires_grad=True)
+    for args in ((many, w), (many, w.detach(), bias)):
+        with pytest.raises(ValueError, match="2\\^22 rows"):
+            ops.f8_linear(*args)
+    with pytest.raises(ValueError, match="2\\^22 columns"):
+        ops.f8_linear(torch.zeros((1, 1), device=cuda).expand(1, (1 << 22) + 1),
+                      torch.zeros((1, 1), device=cuda).expand(1, (1 << 22) + 1))
+
+
+def test_what_the_operators_write_counts_as_modified(cuda):
+    flat = torch.ones((32,), device=cuda)
+    views = [flat[:16], flat[16:]]
+    grads = [torch.ones((16,), device=cuda) for _ in range(2)]
+    for write, touched in ((lambda: ops.clip_norm_(grads, 1.0), grads),
+                           (lambda: ops.clip_norm_(grads, 1.0, out=views), [flat]),
+                           (lambda: ops.clip_norm_(grads, 1.0, out=flat), [flat])):
+        before = [t._version for t in touched]
+        write()
+        assert all(t._version > b for t, b in zip(touched, before))
+    before = [t._version for t in grads]
+    ops.grad_norm(grads)
+    ops.clip_norm_(grads, 1.0, out=flat)
+    assert [t._version for t in grads] == before
+    a = ops.f8_rows(_rows(122, 4, 16).to(cuda))
+    out = torch.ones((4, 4), device=cuda, requires_grad=True).clone()
+    y = out.square()
+    ops.f8_matmul(a, a, out=out.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
