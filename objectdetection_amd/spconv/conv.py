@@ -191,9 +191,14 @@ class SparseConvolution(SparseModule):
         return ops.conv_forward(x, self._weight_image(), rb.out_nbr, rb.k_out, rb.kvol, cin, cout,
                                 scale, shift, relu)
 
+    def __getstate__(self):  # copies and pickles make their own images
+        return {k: v for k, v in self.__dict__.items() if not k.startswith("_wimg")}
+
     def _weight_image(self, planes=0):
         """MFMA weight image (planes 2 / 3: the split bf16x3 / bf16x8 image; "f8": a pointwise conv's
-        8-bit form), cached until the parameter is modified in place or replaced."""
+        8-bit form), cached until the parameter is modified in place or replaced.  The cache holds the
+        values that it was made from, so that their address stays theirs, and an event, for users on
+        another stream; an image made in a graph's capture is that graph's, and is not cached."""
         w = self.weight
         tag = (w.data_ptr(), w._version, w.device, w.dtype)
         name = f"_wimg{planes}"
@@ -204,8 +209,17 @@ class SparseConvolution(SparseModule):
                                           transpose=True)
             else:
                 img = ops.weight_image_bf16x3(w, planes=planes) if planes else ops.weight_image(w)
-            cache = (tag, img)
+            if torch.cuda.is_current_stream_capturing():
+                return img
+            maker = torch.cuda.current_stream(w.device)
+            cache = (tag, img, w.detach(), maker, maker.record_event())
             object.__setattr__(self, name, cache)
+        else:
+            user = torch.cuda.current_stream(w.device)
+            if user != cache[3] and not torch.cuda.is_current_stream_capturing():
+                user.wait_event(cache[4])
+                for t in cache[1] if isinstance(cache[1], tuple) else (cache[1],):
+                    t.record_stream(user)
         return cache[1]
 
 

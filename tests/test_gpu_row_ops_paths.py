@@ -149,3 +149,61 @@ def test_rms_norm_module_is_what_nn_rms_norm_is(cuda):
     b.load_state_dict(a.state_dict())
     x = torch.randn((77, 96), generator=torch.Generator().manual_seed(6)).to(cuda)
     assert torch.allclose(a(x), b(x), rtol=1e-5, atol=1e-6)
+
+
+def test_weight_images_follow_replaced_weights_streams_copies_and_captures(cuda):
+    import copy
+    import io
+    x = _tensor(cuda)
+    feats = x.features
+
+    def run(conv):
+        x.features = feats
+        with torch.no_grad(), ops.conv_math("f8"):
+            return conv(x).features.clone()
+
+    def want(conv):
+        return ops.f8_product(feats, ops.f8_weight_image(conv.weight.detach().view(256, 64), transpose=True))
+    conv = spconv.SubMConv3d(256, 64, 1, bias=False).to(cuda)
+    conv.weight = nn.Parameter(conv.weight.detach().clone())
+    assert torch.equal(run(conv), want(conv))
+    # replaced twice between two calls: the second takes the first one's memory, if that is free
+    conv.weight = nn.Parameter(conv.weight.detach() * 2)
+    conv.weight = nn.Parameter(conv.weight.detach() * 3)
+    assert torch.equal(run(conv), want(conv))
+    # copies and pickles
+    for twin in (copy.deepcopy(conv), torch.load(_saved(conv, io.BytesIO()), weights_only=False)):
+        with torch.no_grad():
+            twin.weight.mul_(0.5)
+        assert torch.equal(run(twin), want(twin))
+    # first used on another stream, then here, and the other way round
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        conv.weight.mul_(2.0)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = run(conv)
+    here = run(conv)
+    torch.cuda.synchronize()
+    assert torch.equal(there, want(conv)) and torch.equal(here, there)
+    # first used in a capture: the graph's image is the graph's
+    run(spconv.SubMConv3d(256, 64, 1, bias=False).to(cuda))
+    with torch.no_grad():
+        conv.weight.mul_(0.25)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(conv)
+    right = want(conv)
+    assert torch.equal(run(conv), right)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, right) and torch.equal(run(conv), right)
+
+
+def _saved(module, file):
+    torch.save(module, file)
+    file.seek(0)
+    return file
