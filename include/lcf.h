@@ -793,6 +793,18 @@ int lcf_f8_linear(const void *x, long long ldx, int dtype, const void *b, long l
                   const float *scale, const float *shift, int relu, void *out, long long ldo,
                   int out_dtype, void *stream);
 
+/* The gradients of a thin layer y = x w^T (+ b) over many rows from one reading of x [R, K] and dy [R, N]:
+ * dw = dy^T x ([N, K], or [K, N] = x^T dy with turned != 0), contiguous, of dw_dtype, both operands in the
+ * columns form of lcf_f8_quant (e4m3) and multiplied as lcf_f8_gemm does for that output type; db [N] =
+ * the columns' sums of dy (NULL = not wanted).  For R >= 4096 and multiples of 8 up to K, N = 128, or one
+ * of them up to 256 and the other up to 64; addresses and strides in whole dwords, strides <= 2^20;
+ * LCF_ERR_UNSUPPORTED otherwise (the workspace is 0 bytes then where sizes are the reason) and the caller
+ * makes the two quantisations and the product. */
+size_t lcf_f8_weight_grad_workspace_bytes(int R, int K, int N);
+int lcf_f8_weight_grad(const void *x, long long ldx, const void *dy, long long lddy, int R, int K, int N,
+                       int dtype, int turned, void *dw, int dw_dtype, void *db, int db_dtype, void *ws,
+                       size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -209,6 +209,9 @@ SYMBOLS = {
     "lcf_f8_linear": (c_int, [c_void_p, c_ll, c_int, c_void_p, c_ll, c_void_p, c_int, c_int, c_int,
                               c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_ll, c_int,
                               c_void_p]),
+    "lcf_f8_weight_grad_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "lcf_f8_weight_grad": (c_int, [c_void_p, c_ll, c_void_p, c_ll, c_int, c_int, c_int, c_int, c_int,
+                                   c_void_p, c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "lcf_f8_gemm": (c_int, [c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_ll, c_void_p,
                             c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
                             c_void_p, c_ll, c_int, c_void_p, c_size_t, c_void_p]),

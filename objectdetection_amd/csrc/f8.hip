@@ -1182,3 +1182,308 @@ extern "C" int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa
     }
     return LCF_OK;
 }
+
+// ---------------------------------------------------------------- a thin layer's weight gradient
+// out [M, N] = A^T B for A [R, M] and B [R, N] of fp32 / bf16 / fp16, both brought into columns form
+// (blocks of 128 rows of a column) on the way: one reading of each and nothing written but the sums.
+// A workgroup takes 128 rows at a time.  A wave holds 32 columns of them, a lane 8 rows x 8 columns
+// (rl, cl): a column's largest magnitude is the lane's own rows and four lane swaps, without a barrier.
+// The bytes are turned into LDS (a column's 128 rows, one behind the other, columns 144 bytes apart:
+// 16 columns start in 16 different sets of four banks), and the next 128 rows are asked for before the
+// products of these, 32 x 64 outputs a wave, begin.  Rows behind R read as zeros (offsets past the
+// buffer's end).  As many workgroups as there are compute units and a few more, each with its own sums,
+// joined in a fixed order.
+#define F8_TURN 144
+struct F8Wgrad {
+    const unsigned char *a, *b;
+    float *parts, *sums; // [workgroups][M][N]; [workgroups][width of the summed side] or NULL
+    long long lda, ldb;
+    int R, M, N, steps, sum_a; // steps: blocks of 128 rows of a workgroup
+};
+
+typedef unsigned short f8_h2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned f8_max16(unsigned a, unsigned b)
+{
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(f8_h2, a), __builtin_bit_cast(f8_h2, b)));
+}
+
+template <typename T, bool WIDE, int MC, int NC> // MC, NC: 64 columns of A, of B
+__global__ void __launch_bounds__(128 * (MC + NC), 3) f8_wgrad_kernel(F8Wgrad p)
+{
+    constexpr int E = sizeof(T), D = 2 * E; // dwords of eight columns
+    __shared__ __align__(16) unsigned char turn[64 * (MC + NC) * F8_TURN];
+    __shared__ __align__(8) unsigned char exps[64 * (MC + NC)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cl = lane & 3, rl = lane >> 2, r16 = lane & 15, g = lane >> 4;
+    const int mine = wave < 2 * MC * NC ? wave : 0;
+    const bool of_b = wave >= 2 * MC;
+    const int col = (of_b ? wave - 2 * MC : wave) * 32 + cl * 8, width = of_b ? p.N : p.M;
+    const int ld = (int)(of_b ? p.ldb : p.lda);
+    const unsigned char *src = of_b ? p.b : p.a;
+    const bool summed = p.sums && (p.sum_a != 0) == !of_b;
+    const int off = col < width ? (rl * 8 * ld + col) * E : (int)0x80000000;
+    unsigned v[8][D];
+    auto ask = [&](int block) {
+        const int left = min(p.R - block * 128, 128);
+        const __amdgpu_buffer_rsrc_t buf = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<unsigned char *>(src + (long long)block * 128 * ld * E), 0, ((left - 1) * ld + width) * E, 0x00020000);
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int d = 0; d < D; d += 4) {
+                const u4 q = __builtin_amdgcn_raw_buffer_load_b128(buf, off + i * ld * E + d * 4, 0, 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[i][d + k] = q[k];
+            }
+    };
+    auto value = [&](int i, int j) -> float {
+        if constexpr (E == 4) return __uint_as_float(v[i][j]);
+        else return lcf_to_f32(__builtin_bit_cast(T, (unsigned short)(v[i][j >> 1] >> (16 * (j & 1)))));
+    };
+    f8_f4 acc[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[i][t] = (f8_f4){0.f, 0.f, 0.f, 0.f};
+    __shared__ float totals[64 * (MC + NC)]; // a wave's own 32 columns
+    if (lane < 32) totals[wave * 32 + lane] = 0.f;
+
+    const int blocks = (p.R + 127) >> 7, first = blockIdx.x * p.steps, last = min(first + p.steps, blocks);
+    ask(first);
+    for (int block = first; block < last; ++block) {
+        if (summed) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += value(i, j);
+#pragma unroll
+                for (int x = 4; x <= 32; x <<= 1) s += __shfl_xor(s, x, 64);
+                if (rl == 0) totals[wave * 32 + cl * 8 + j] += s;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // the columns' largest finite magnitudes; infinities become NaN where one is found
+        float top[8];
+        if constexpr (E == 2) {
+            constexpr unsigned INF = __is_same(T, lcf_b) ? 0x7F80u : 0x7C00u;
+            unsigned m[4];
+            // magnitudes of 16 bits order as whole numbers do
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                m[d] = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m[d] = f8_max16(m[d], v[i][d] & 0x7FFF7FFFu);
+            }
+            const unsigned all = f8_max16(f8_max16(m[0], m[1]), f8_max16(m[2], m[3]));
+            if (__builtin_expect(__any((all & 0xFFFF) >= INF || (all >> 16) >= INF), 0)) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    m[d] = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        unsigned u = v[i][d] & 0x7FFF7FFFu;
+                        if ((u & 0xFFFF) >= INF) { v[i][d] |= 0x7FFFu; u &= 0xFFFF0000u; }
+                        if ((u >> 16) >= INF) { v[i][d] |= 0x7FFF0000u; u &= 0xFFFFu; }
+                        m[d] = f8_max16(m[d], u);
+                    }
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+#pragma unroll
+                for (int x = 4; x <= 32; x <<= 1) m[d] = f8_max16(m[d], (unsigned)__shfl_xor((int)m[d], x, 64));
+                top[2 * d] = lcf_to_f32(__builtin_bit_cast(T, (unsigned short)(m[d] & 0xFFFF)));
+                top[2 * d + 1] = lcf_to_f32(__builtin_bit_cast(T, (unsigned short)(m[d] >> 16)));
+            }
+        } else {
+            float all = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                top[j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top[j] = fmaxf(top[j], __builtin_fabsf(value(i, j)));
+                all = fmaxf(all, top[j]);
+            }
+            if (__builtin_expect(__any(all > 3.402823466e38f), 0)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    top[j] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (__builtin_fabsf(value(i, j)) > 3.402823466e38f) v[i][j] = 0x7FC00000u;
+                        top[j] = fmaxf(top[j], __builtin_fabsf(value(i, j)));
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int x = 4; x <= 32; x <<= 1) top[j] = fmaxf(top[j], __shfl_xor(top[j], x, 64));
+        }
+        if (block != first) __syncthreads(); // the last products have read their bytes
+        unsigned e4[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int e = lcf_f8_exponent(top[j], LCF_E4M3);
+            const float s = lcf_exp2i(-e);
+            e4[j >> 2] |= (unsigned)(e + 127) << (8 * (j & 3));
+            lcf_u2u w;
+            w.x = lcf_f8_pack4(value(0, j) * s, value(1, j) * s, value(2, j) * s, value(3, j) * s, LCF_E4M3);
+            w.y = lcf_f8_pack4(value(4, j) * s, value(5, j) * s, value(6, j) * s, value(7, j) * s, LCF_E4M3);
+            *reinterpret_cast<uint2 *>(turn + (wave * 32 + cl * 8 + j) * F8_TURN + rl * 8) = make_uint2(w.x, w.y);
+            __builtin_amdgcn_sched_barrier(0); // one column at a time: all at once would not fit the registers
+        }
+        if (rl == 0) *reinterpret_cast<uint2 *>(exps + wave * 32 + cl * 8) = make_uint2(e4[0], e4[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (block + 1 < last) ask(block + 1);
+        __syncthreads();
+        { // (waves that have no outputs of their own make the first one's: around a branch the sums would
+          // be held twice)
+            const int m0 = mine % (2 * MC) * 32 + r16, n0 = 64 * MC + mine / (2 * MC) * 64 + r16;
+            auto bytes = [&](int c) -> f8_v8 {
+                const f8_v4 *t = reinterpret_cast<const f8_v4 *>(turn + c * F8_TURN + g * 32);
+                const f8_v4 lo = t[0], hi = t[1];
+                return (f8_v8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            if constexpr (WIDE) { // few registers are left beside the rows asked for: 16 of a lane's 32 bytes at a time
+                auto wide = [&](int c, int k, f8_b8 *w) {
+                    const f8_v4 q = *reinterpret_cast<const f8_v4 *>(turn + c * F8_TURN + g * 32 + k * 16);
+                    const float s = lcf_exp2i((int)exps[c] - 127);
+                    w[0] = f8_to_bf16<LCF_E4M3>(q[0], q[1], s);
+                    w[1] = f8_to_bf16<LCF_E4M3>(q[2], q[3], s);
+                };
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    f8_b8 wa[2][2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) wide(m0 + i * 16, k, wa[i]);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        f8_b8 wb[2];
+                        wide(n0 + t * 16, k, wb);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[h], wa[i][h], acc[i][t], 0, 0, 0);
+                        if (t == 1 || t == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            } else {
+                f8_v8 qa[2];
+                int ea[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    qa[i] = bytes(m0 + i * 16);
+                    ea[i] = exps[m0 + i * 16];
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const f8_v8 qb = bytes(n0 + t * 16);
+                    const int eb = exps[n0 + t * 16];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(qb, qa[i], acc[i][t], LCF_E4M3, LCF_E4M3,
+                                                                                     0, eb, 0, ea[i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) f8_pin(acc[i]);
+    if (wave < 2 * MC * NC) {
+        float *o = p.parts + (long long)blockIdx.x * p.M * p.N;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int m = wave % (2 * MC) * 32 + i * 16 + r16, n = wave / (2 * MC) * 64 + t * 16 + 4 * g;
+                if (m < p.M && n < p.N)
+                    *reinterpret_cast<lcf_f4u *>(o + (long long)m * p.N + n) =
+                        (lcf_f4u){acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
+            }
+    }
+    if (summed && lane < 32 && col - cl * 8 + lane < width)
+        p.sums[(long long)blockIdx.x * width + col - cl * 8 + lane] = totals[wave * 32 + lane];
+}
+
+// columns of 64 of either side that one of the kernel's forms holds: a < 0 where none does
+struct F8WgradShape {
+    int a, b, parts, steps;
+};
+static F8WgradShape f8_wgrad_shape(int R, int M, int N)
+{
+    F8WgradShape s{-1, -1, 0, 0};
+    // sums over fewer rows are split over the chip by the columns forms and their product as well
+    if (R < 4096 || R > F8_MOST || M < 8 || N < 8 || (M & 7) || (N & 7)) return s;
+    if (M <= 64 && N <= 64) s.a = 1, s.b = 1;
+    else if (M <= 128 && N <= 128) s.a = 2, s.b = 2;
+    else if (M <= 256 && N <= 64) s.a = 4, s.b = 1;
+    else if (M <= 64 && N <= 256) s.a = 1, s.b = 4;
+    else return s;
+    const int blocks = (R + 127) / 128;
+    s.steps = (blocks + 255) / 256;
+    s.parts = (blocks + s.steps - 1) / s.steps;
+    return s;
+}
+
+template <typename T, bool WIDE> static void f8_wgrad_launch(const F8Wgrad &p, const F8WgradShape &s, hipStream_t st)
+{
+    if (s.a == 1 && s.b == 1) f8_wgrad_kernel<T, WIDE, 1, 1><<<s.parts, 256, 0, st>>>(p);
+    else if (s.a == 2) f8_wgrad_kernel<T, WIDE, 2, 2><<<s.parts, 512, 0, st>>>(p);
+    else if (s.a == 4) f8_wgrad_kernel<T, WIDE, 4, 1><<<s.parts, 640, 0, st>>>(p);
+    else f8_wgrad_kernel<T, WIDE, 1, 4><<<s.parts, 640, 0, st>>>(p);
+}
+
+extern "C" size_t lcf_f8_weight_grad_workspace_bytes(int R, int K, int N)
+{
+    const F8WgradShape s = f8_wgrad_shape(R, K, N);
+    return s.a < 0 ? 0 : (size_t)s.parts * ((size_t)K * N + N) * sizeof(float);
+}
+
+extern "C" int lcf_f8_weight_grad(const void *x, long long ldx, const void *dy, long long lddy, int R, int K, int N,
+                                  int dtype, int turned, void *dw, int dw_dtype, void *db, int db_dtype, void *ws,
+                                  size_t ws_bytes, void *stream)
+{
+    if (R < 0 || K < 0 || N < 0 || !lcf_is_type(dtype) || !lcf_is_type(dw_dtype) || (db && !lcf_is_type(db_dtype)))
+        return LCF_ERR_ARG;
+    const F8WgradShape s = turned ? f8_wgrad_shape(R, K, N) : f8_wgrad_shape(R, N, K);
+    if (s.a < 0) return LCF_ERR_UNSUPPORTED;
+    if (!x || !dy || !dw || ldx < K || lddy < N) return LCF_ERR_ARG;
+    // rows are read 16 bytes at a time by buffer loads that want four-byte addresses and 32-bit offsets
+    const int e = lcf_type_size(dtype);
+    if (((uintptr_t)x & 3) || ((uintptr_t)dy & 3) || (ldx * e & 3) || (lddy * e & 3) || ldx > 1 << 20 || lddy > 1 << 20)
+        return LCF_ERR_UNSUPPORTED;
+    if (!ws) return LCF_ERR_ARG;
+    if (ws_bytes < lcf_f8_weight_grad_workspace_bytes(R, K, N)) return LCF_ERR_WORKSPACE;
+    F8Wgrad p{};
+    p.a = (const unsigned char *)(turned ? x : dy);
+    p.lda = turned ? ldx : lddy;
+    p.b = (const unsigned char *)(turned ? dy : x);
+    p.ldb = turned ? lddy : ldx;
+    p.M = turned ? K : N;
+    p.N = turned ? N : K;
+    p.R = R;
+    p.steps = s.steps;
+    p.parts = (float *)ws;
+    p.sums = db ? p.parts + (size_t)s.parts * K * N : nullptr;
+    p.sum_a = !turned;
+    hipStream_t st = (hipStream_t)stream;
+    const bool wide = dw_dtype == LCF_F32;
+    if (dtype == LCF_F32) wide ? f8_wgrad_launch<float, true>(p, s, st) : f8_wgrad_launch<float, false>(p, s, st);
+    else if (dtype == LCF_BF16) wide ? f8_wgrad_launch<lcf_b, true>(p, s, st) : f8_wgrad_launch<lcf_b, false>(p, s, st);
+    else wide ? f8_wgrad_launch<lcf_h, true>(p, s, st) : f8_wgrad_launch<lcf_h, false>(p, s, st);
+    LCF_CHECK_LAUNCH();
+    F8Gemm j{};
+    j.ws = p.parts;
+    j.out = dw;
+    j.ldo = p.N;
+    j.code = dw_dtype;
+    j.M = p.M;
+    j.N = p.N;
+    f8_join_kernel<<<(unsigned)((K * N + 63) / 64), 256, 0, st>>>(j, s.parts);
+    LCF_CHECK_LAUNCH();
+    return db ? lcf_sum_parts(p.sums, s.parts, N, db, db_dtype, stream) : LCF_OK;
+}

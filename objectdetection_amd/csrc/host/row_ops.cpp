@@ -29,7 +29,8 @@ struct Err : std::runtime_error {
 
 #define LCF_FUNCTIONS(F)                                                                                       \
     F(strerror) F(grad_norm_workspace_bytes) F(grad_norm) F(grad_clip) F(rms_norm_fwd) F(rms_norm_workspace_bytes) \
-    F(rms_norm_bwd) F(f8_quant) F(f8_gemm_workspace_bytes) F(f8_gemm) F(f8_linear) F(sum_parts)
+    F(rms_norm_bwd) F(f8_quant) F(f8_gemm_workspace_bytes) F(f8_gemm) F(f8_linear) F(sum_parts) \
+    F(f8_weight_grad_workspace_bytes) F(f8_weight_grad)
 struct Lib {
 #define F(name) decltype(&lcf_##name) name;
     LCF_FUNCTIONS(F)
@@ -494,6 +495,25 @@ Tensor f8_linear_fwd(const Tensor &x, const Tensor &w, const Tensor *bias, bool 
     return f8_mm(*x8, image, nullptr, sh, false, type_code(x.scalar_type()), nullptr, on.st);
 }
 
+// dw and, with bias >= 0, db of that type, where lcf_f8_weight_grad takes the sizes; false elsewhere
+bool f8_weight_grad(const Tensor &x, const Tensor &dy, bool turned, const Tensor &w, int bias, Tensor &dw, Tensor &db, void *st)
+{
+    const int R = count(x.size(0), "f8_linear"), K = count(x.size(1), "f8_linear"), N = count(dy.size(1), "f8_linear");
+    const size_t n = L.f8_weight_grad_workspace_bytes(R, K, N);
+    if (!n) return false;
+    const Rows xv = rows_of(x, K), dv = rows_of(dy, N);
+    const Tensor ws = bytes(n, x), to = at::empty(w.sizes(), w.options()),
+                 sum = bias >= 0 ? at::empty({N}, x.options().dtype(type_of(bias))) : Tensor();
+    const int rc = L.f8_weight_grad(xv.ptr(), xv.ld, dv.ptr(), dv.ld, R, K, N, type_code(x.scalar_type()), turned,
+                                    to.data_ptr(), type_code(w.scalar_type()), bias >= 0 ? sum.data_ptr() : nullptr,
+                                    bias >= 0 ? bias : 0, ws.data_ptr(), (size_t)ws.numel(), st);
+    if (rc == LCF_ERR_UNSUPPORTED) return false;
+    check(rc);
+    dw = to;
+    db = sum;
+    return true;
+}
+
 // y = x W^T (+ bias) with x and W rounded to 8-bit form.  The three products (y, dx = dy W, dW = dy^T x)
 // run on 8-bit operands, each operand's scale blocks lying along the axis that its product sums over;
 // the rounding is passed through unchanged.  turned: the weight is stored [K, N].
@@ -516,8 +536,8 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
         const Tensor &x = saved[0], &w = saved[1];
         const bool turned = ctx->saved_data["turned"].toBool();
         const int bias = (int)ctx->saved_data["bias"].toInt();
-        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
-                   need_b = bias >= 0 && ctx->needs_input_grad(2);
+        const bool need_x = ctx->needs_input_grad(0);
+        bool need_w = ctx->needs_input_grad(1), need_b = bias >= 0 && ctx->needs_input_grad(2);
         const On on(x);
         Tensor dy = grads[0], dx, dw, db;
         if (dy.scalar_type() != x.scalar_type()) dy = dy.to(x.scalar_type());
@@ -528,7 +548,12 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
             image = f8_operand(saved[2], saved[3], "weight");
             dx = f8_fused(dy, image, nullptr, nullptr, false, on.st);
         }
+        // the weight's gradient and the bias's take both as they are where one kernel does all
+        bool done = false;
+        if (need_w) done = f8_weight_grad(x, dy, turned, w, need_b ? bias : -1, dw, db, on.st);
         const bool rows = need_x && !dx.defined();
+        need_w = need_w && !done;
+        need_b = need_b && !done;
         Quant q;
         if (rows || need_w || need_b) q = f8_quant(dy, LCF_E4M3, false, rows, need_w, need_b, on.st);
         if (rows) dx = f8_mm(q.rows, image, nullptr, nullptr, false, type_code(dy.scalar_type()), nullptr, on.st);
