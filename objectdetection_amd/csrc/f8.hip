@@ -963,7 +963,7 @@ __global__ void __launch_bounds__(256) f8_join_kernel(F8Gemm p, int splits)
     const int part = threadIdx.x & 15, line = threadIdx.x >> 4;
     const long long e = (long long)blockIdx.x * 64 + part * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
     for (int s = line; s < splits; s += 16) {
         const float *o = p.ws + s * total + e;
         if (e + 4 <= total) {
@@ -1416,8 +1416,7 @@ struct F8WgradShape {
 static F8WgradShape f8_wgrad_shape(int R, int M, int N)
 {
     F8WgradShape s{-1, -1, 0, 0};
-    // sums over fewer rows are split over the chip by the columns forms and their product as well
-    if (R < 4096 || R > F8_MOST || M < 8 || N < 8 || (M & 7) || (N & 7)) return s;
+    if (R < 1 || R > F8_MOST || M < 8 || N < 8 || (M & 7) || (N & 7)) return s;
     if (M <= 64 && N <= 64) s.a = 1, s.b = 1;
     else if (M <= 128 && N <= 128) s.a = 2, s.b = 2;
     else if (M <= 256 && N <= 64) s.a = 4, s.b = 1;
