@@ -796,8 +796,8 @@ int lcf_f8_linear(const void *x, long long ldx, int dtype, const void *b, long l
 /* The gradients of a thin layer y = x w^T (+ b) over many rows from one reading of x [R, K] and dy [R, N]:
  * dw = dy^T x ([N, K], or [K, N] = x^T dy with turned != 0), contiguous, of dw_dtype, both operands in the
  * columns form of lcf_f8_quant (e4m3) and multiplied as lcf_f8_gemm does for that output type; db [N] =
- * the columns' sums of dy (NULL = not wanted).  For R >= 1 and multiples of 8 up to K, N = 128, or one
- * of them up to 256 and the other up to 64; addresses and strides in whole dwords, strides <= 2^20;
+ * the columns' sums of dy (NULL = not wanted).  For R >= 1, K and N multiples of 8 up to 256,
+ * addresses and strides in whole dwords, strides <= 2^20;
  * LCF_ERR_UNSUPPORTED otherwise (the workspace is 0 bytes then where sizes are the reason) and the caller
  * makes the two quantisations and the product. */
 size_t lcf_f8_weight_grad_workspace_bytes(int R, int K, int N);

@@ -1191,9 +1191,14 @@ extern "C" int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa
 // The bytes are turned into LDS (a column's 128 rows, one behind the other, columns 144 bytes apart:
 // 16 columns start in 16 different sets of four banks), and the next 128 rows are asked for before the
 // products of these, 32 x 64 outputs a wave, begin.  Rows behind R read as zeros (offsets past the
-// buffer's end).  As many workgroups as there are compute units and a few more, each with its own sums,
-// joined in a fixed order.
+// buffer's end).  As many workgroups as there are compute units, each with its own sums, joined in a
+// fixed order.  Bound by memory: 136000 rows, 64 x 256, bf16 25 us (3.5 TB/s; a unit waits while it
+// turns), fp32 36 us (4.8 TB/s), and 3 us for the join; the two columns forms, their product and its
+// join took 59 us.  Outputs of 256 columns are kept whole beside 64 of the other side, where dividing
+// them in two takes 28 us; 256 x 256 is made in four parts (136000 rows 57 us).  Beyond that each part
+// reads its sides again and the columns forms take over.
 #define F8_TURN 144
+#define F8_SLOTS 256 // workgroups of a launch: 384 take 30 us and 192 28 us where 256 take 25
 struct F8Wgrad {
     const unsigned char *a, *b;
     float *parts, *sums; // [workgroups][M][N]; [workgroups][width of the summed side] or NULL
@@ -1208,7 +1213,7 @@ __device__ __forceinline__ unsigned f8_max16(unsigned a, unsigned b)
 }
 
 template <typename T, bool WIDE, int MC, int NC> // MC, NC: 64 columns of A, of B
-__global__ void __launch_bounds__(128 * (MC + NC), 3) f8_wgrad_kernel(F8Wgrad p)
+__global__ void __launch_bounds__(128 * (MC + NC), sizeof(T) == 2 && MC + NC < 5 ? 4 : 3) f8_wgrad_kernel(F8Wgrad p)
 {
     constexpr int E = sizeof(T), D = 2 * E; // dwords of eight columns
     __shared__ __align__(16) unsigned char turn[64 * (MC + NC) * F8_TURN];
@@ -1217,10 +1222,11 @@ __global__ void __launch_bounds__(128 * (MC + NC), 3) f8_wgrad_kernel(F8Wgrad p)
     const int cl = lane & 3, rl = lane >> 2, r16 = lane & 15, g = lane >> 4;
     const int mine = wave < 2 * MC * NC ? wave : 0;
     const bool of_b = wave >= 2 * MC;
-    const int col = (of_b ? wave - 2 * MC : wave) * 32 + cl * 8, width = of_b ? p.N : p.M;
+    const int a0 = blockIdx.y * 64 * MC, b0 = blockIdx.z * 64 * NC; // the workgroup's first columns
+    const int col = of_b ? b0 + (wave - 2 * MC) * 32 + cl * 8 : a0 + wave * 32 + cl * 8, width = of_b ? p.N : p.M;
     const int ld = (int)(of_b ? p.ldb : p.lda);
     const unsigned char *src = of_b ? p.b : p.a;
-    const bool summed = p.sums && (p.sum_a != 0) == !of_b;
+    const bool summed = p.sums && (p.sum_a ? !of_b && blockIdx.z == 0 : of_b && blockIdx.y == 0);
     const int off = col < width ? (rl * 8 * ld + col) * E : (int)0x80000000;
     unsigned v[8][D];
     auto ask = [&](int block) {
@@ -1399,7 +1405,7 @@ __global__ void __launch_bounds__(128 * (MC + NC), 3) f8_wgrad_kernel(F8Wgrad p)
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const int m = wave % (2 * MC) * 32 + i * 16 + r16, n = wave / (2 * MC) * 64 + t * 16 + 4 * g;
+                const int m = a0 + wave % (2 * MC) * 32 + i * 16 + r16, n = b0 + wave / (2 * MC) * 64 + t * 16 + 4 * g;
                 if (m < p.M && n < p.N)
                     *reinterpret_cast<lcf_f4u *>(o + (long long)m * p.N + n) =
                         (lcf_f4u){acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
@@ -1409,37 +1415,34 @@ __global__ void __launch_bounds__(128 * (MC + NC), 3) f8_wgrad_kernel(F8Wgrad p)
         p.sums[(long long)blockIdx.x * width + col - cl * 8 + lane] = totals[wave * 32 + lane];
 }
 
-// columns of 64 of either side that one of the kernel's forms holds: a < 0 where none does
-struct F8WgradShape {
-    int a, b, parts, steps;
+struct F8WgradShape { // parts = 0: sizes that the kernel does not take
+    int a, b, parts, steps; // a, b: columns of either side in a workgroup, in 64
 };
 static F8WgradShape f8_wgrad_shape(int R, int M, int N)
 {
-    F8WgradShape s{-1, -1, 0, 0};
-    if (R < 1 || R > F8_MOST || M < 8 || N < 8 || (M & 7) || (N & 7)) return s;
-    if (M <= 64 && N <= 64) s.a = 1, s.b = 1;
-    else if (M <= 128 && N <= 128) s.a = 2, s.b = 2;
-    else if (M <= 256 && N <= 64) s.a = 4, s.b = 1;
-    else if (M <= 64 && N <= 256) s.a = 1, s.b = 4;
-    else return s;
-    const int blocks = (R + 127) / 128;
-    s.steps = (blocks + 255) / 256;
+    F8WgradShape s{M <= 64 ? 1 : M <= 128 || N > 64 ? 2 : 4, N <= 64 ? 1 : N <= 128 || M > 64 ? 2 : 4, 0, 0};
+    if (R < 1 || R > F8_MOST || M < 8 || N < 8 || (M & 7) || (N & 7) || M > 256 || N > 256) return s;
+    const int blocks = (R + 127) / 128, groups = (M + 64 * s.a - 1) / (64 * s.a) * ((N + 64 * s.b - 1) / (64 * s.b));
+    s.steps = ((long long)blocks * groups + F8_SLOTS - 1) / F8_SLOTS;
     s.parts = (blocks + s.steps - 1) / s.steps;
     return s;
 }
 
 template <typename T, bool WIDE> static void f8_wgrad_launch(const F8Wgrad &p, const F8WgradShape &s, hipStream_t st)
 {
-    if (s.a == 1 && s.b == 1) f8_wgrad_kernel<T, WIDE, 1, 1><<<s.parts, 256, 0, st>>>(p);
-    else if (s.a == 2) f8_wgrad_kernel<T, WIDE, 2, 2><<<s.parts, 512, 0, st>>>(p);
-    else if (s.a == 4) f8_wgrad_kernel<T, WIDE, 4, 1><<<s.parts, 640, 0, st>>>(p);
-    else f8_wgrad_kernel<T, WIDE, 1, 4><<<s.parts, 640, 0, st>>>(p);
+    const dim3 grid(s.parts, (p.M + 64 * s.a - 1) / (64 * s.a), (p.N + 64 * s.b - 1) / (64 * s.b));
+    if (s.a == 1 && s.b == 1) f8_wgrad_kernel<T, WIDE, 1, 1><<<grid, 256, 0, st>>>(p);
+    else if (s.a == 2 && s.b == 1) f8_wgrad_kernel<T, WIDE, 2, 1><<<grid, 384, 0, st>>>(p);
+    else if (s.a == 1 && s.b == 2) f8_wgrad_kernel<T, WIDE, 1, 2><<<grid, 384, 0, st>>>(p);
+    else if (s.a == 4) f8_wgrad_kernel<T, WIDE, 4, 1><<<grid, 640, 0, st>>>(p);
+    else if (s.b == 4) f8_wgrad_kernel<T, WIDE, 1, 4><<<grid, 640, 0, st>>>(p);
+    else f8_wgrad_kernel<T, WIDE, 2, 2><<<grid, 512, 0, st>>>(p);
 }
 
 extern "C" size_t lcf_f8_weight_grad_workspace_bytes(int R, int K, int N)
 {
     const F8WgradShape s = f8_wgrad_shape(R, K, N);
-    return s.a < 0 ? 0 : (size_t)s.parts * ((size_t)K * N + N) * sizeof(float);
+    return s.parts == 0 ? 0 : (size_t)s.parts * ((size_t)K * N + N) * sizeof(float);
 }
 
 extern "C" int lcf_f8_weight_grad(const void *x, long long ldx, const void *dy, long long lddy, int R, int K, int N,
@@ -1449,7 +1452,7 @@ extern "C" int lcf_f8_weight_grad(const void *x, long long ldx, const void *dy, 
     if (R < 0 || K < 0 || N < 0 || !lcf_is_type(dtype) || !lcf_is_type(dw_dtype) || (db && !lcf_is_type(db_dtype)))
         return LCF_ERR_ARG;
     const F8WgradShape s = turned ? f8_wgrad_shape(R, K, N) : f8_wgrad_shape(R, N, K);
-    if (s.a < 0) return LCF_ERR_UNSUPPORTED;
+    if (s.parts == 0) return LCF_ERR_UNSUPPORTED;
     if (!x || !dy || !dw || ldx < K || lddy < N) return LCF_ERR_ARG;
     // rows are read 16 bytes at a time by buffer loads that want four-byte addresses and 32-bit offsets
     const int e = lcf_type_size(dtype);

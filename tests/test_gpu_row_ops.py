@@ -711,3 +711,54 @@ def test_what_the_operators_write_counts_as_modified(cuda):
     ops.f8_matmul(a, a, out=out.detach())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 8, 8), (127, 64, 64), (129, 72, 24), (257, 128, 40), (500, 40, 136), (3000, 256, 64),
+                                   (1300, 64, 256), (700, 200, 144), (33000, 256, 256), (66000, 32, 200)])
+def test_f8_linear_weight_and_bias_gradient_in_one_reading(cuda, shape, dtype):
+    R, K, N = shape
+    assert ops._lib.lib().lcf_f8_weight_grad_workspace_bytes(R, K, N) > 0
+    x, dy = _rows(130, R, K, dtype), _rows(131, R, N, dtype, 1e-2)
+    dt, xt = ref.value(*ref.quantise(dy.t())), ref.value(*ref.quantise(x.t()))
+    want, sums = dt @ xt.t(), dy.double().sum(0)
+    for wtype, turned in ((torch.float32, False), (torch.float32, True), (torch.bfloat16, True), (torch.float16, False)):
+        w = _rows(132, N, K, size=K ** -0.5).to(wtype)
+        w = (w.t().contiguous() if turned else w).to(cuda).requires_grad_()
+        bias = torch.zeros((N,), dtype=wtype, device=cuda, requires_grad=True)
+        y = ops.f8_linear(x.to(cuda), w, bias, turned)
+        dw, db = torch.autograd.grad(y, (w, bias), dy.to(cuda))
+        again = torch.autograd.grad(ops.f8_linear(x.to(cuda), w, bias, turned), (w, bias), dy.to(cuda))
+        assert dw.dtype == wtype and torch.equal(dw, again[0]) and torch.equal(db, again[1])
+        _within(dw.t() if turned else dw, want, _product_bound(dt, xt, R, want, wtype) + tiny(wtype), "dw")
+        # 128 rows of a block one behind the other, the blocks of a workgroup, then 64 bits
+        _within(db, sums, (140 + R // 128) * F32 * dy.double().abs().sum(0) + half_step(wtype) * 1.01 * sums.abs()
+                + tiny(wtype), "db")
+        only, = torch.autograd.grad(ops.f8_linear(x.to(cuda), w, None, turned), w, dy.to(cuda))
+        assert torch.equal(only, dw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_f8_linear_weight_gradient_of_strided_and_unfinished_rows(cuda, dtype):
+    R, K, N = 400, 64, 128
+    room = torch.full((R, K + 24), float("nan"), dtype=dtype, device=cuda)
+    room[:, 8:8 + K] = _rows(133, R, K, dtype).to(cuda)
+    grads = torch.full((R, N + 3), float("nan"), dtype=dtype, device=cuda)
+    grads[:, 1:1 + N] = _rows(134, R, N, dtype).to(cuda)
+    w = torch.zeros((N, K), device=cuda, requires_grad=True)
+
+    def grad(x, dy):
+        return torch.autograd.grad(ops.f8_linear(x, w), w, dy)[0]
+    want = grad(room[:, 8:8 + K].contiguous(), grads[:, 1:1 + N].contiguous())
+    assert bool(want.isfinite().all())
+    assert torch.equal(grad(room[:, 8:8 + K], grads[:, 1:1 + N].contiguous()), want)
+    # rows that do not start on whole dwords take the columns forms: the same products in another order
+    odd = grad(room[:, 8:8 + K], grads[:, 1:1 + N])
+    assert (odd - want).abs().max() <= 1e-5 * want.abs().max()
+    # an infinity or a NaN reaches its own row or column of the gradient and no other
+    x, dy = room[:, 8:8 + K].contiguous(), grads[:, 1:1 + N].contiguous()
+    x[5, 3], x[300, 17], dy[130, 9] = float("inf"), float("nan"), float("-inf")
+    got = grad(x, dy)
+    bad = torch.zeros((N, K), dtype=torch.bool, device=cuda)
+    bad[:, 3] = bad[:, 17] = bad[9] = True
+    assert bool(got[bad].isnan().all()) and bool(got[~bad].isfinite().all())

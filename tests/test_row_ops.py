@@ -134,3 +134,20 @@ def test_abi_refuses_bad_8_bit_operands():
         assert gemm(**big) == UNSUPPORTED, big
     assert L.lcf_f8_gemm_workspace_bytes(last, last, 64, 0) == 0
     assert gemm(M=0, a=None) == 0 and gemm(N=0, b=None) == 0
+
+
+def test_abi_refuses_bad_weight_gradients():
+    L = _lib.lib()
+
+    def grad(x=4096, ldx=64, dy=8192, lddy=32, R=100, K=64, N=32, dt=0, turned=0, dw=12288, dwt=0, db=None, dbt=0,
+             ws=16384, n=1 << 30):
+        return L.lcf_f8_weight_grad(x, ldx, dy, lddy, R, K, N, dt, turned, dw, dwt, db, dbt, ws, n, None)
+    for bad in (dict(x=None), dict(dy=None), dict(dw=None), dict(ldx=60), dict(lddy=31), dict(R=-1), dict(K=-8),
+                dict(dt=3), dict(dwt=-1), dict(db=4096, dbt=3), dict(ws=None)):
+        assert grad(**bad) == ARG, bad
+    for other in (dict(R=0), dict(K=60), dict(N=33, lddy=33), dict(K=264, ldx=264), dict(N=512, lddy=512), dict(x=4098),
+                  dict(dt=1, ldx=65), dict(lddy=(1 << 20) + 4)):
+        assert grad(**other) == UNSUPPORTED, other
+    assert grad(n=100) == WORKSPACE
+    assert L.lcf_f8_weight_grad_workspace_bytes(100, 60, 32) == 0
+    assert L.lcf_f8_weight_grad_workspace_bytes(100, 64, 32) >= (64 * 32 + 32) * 4
