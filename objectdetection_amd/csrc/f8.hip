@@ -1193,7 +1193,7 @@ extern "C" int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa
 // products of these, 32 x 64 outputs a wave, begin.  Rows behind R read as zeros (offsets past the
 // buffer's end).  As many workgroups as there are compute units, each with its own sums, joined in a
 // fixed order.  Bound by memory: 136000 rows, 64 x 256, bf16 25 us (3.5 TB/s; a unit waits while it
-// turns), fp32 36 us (4.8 TB/s), and 3 us for the join; the two columns forms, their product and its
+// turns), fp32 36 us (4.8 TB/s), and 6 us for the join; the two columns forms, their product and its
 // join took 59 us.  Outputs of 256 columns are kept whole beside 64 of the other side, where dividing
 // them in two takes 28 us; 256 x 256 is made in four parts (136000 rows 57 us).  Beyond that each part
 // reads its sides again and the columns forms take over.
