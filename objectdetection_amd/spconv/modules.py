@@ -38,17 +38,17 @@ class RMSNorm(nn.RMSNorm):
     SparseSequential it runs on ``.features``), optionally with the residual's addition of a
     SparseBasicBlock (second/pytorch/models/resnet.py:54-64): ``norm(x, residual)`` ->
     (normed, x + residual).  Statistics are per row, so unlike BatchNorm1d it does the same in
-    training and inference and for any number of rows.  eps None: the rows' type's epsilon, as in
-    nn.RMSNorm."""
+    training and inference and for any number of rows.  eps None: 2^-23, float32's epsilon, for rows of
+    every type, which is what nn.RMSNorm computes (the sums are float32's whatever the rows' type)."""
 
     def __init__(self, num_features, eps=None, elementwise_affine=True):
         super().__init__(num_features, eps, elementwise_affine)
 
-    def _eps(self, x):
-        return torch.finfo(x.dtype).eps if self.eps is None else self.eps
+    def _eps(self):
+        return torch.finfo(torch.float32).eps if self.eps is None else self.eps
 
     def forward(self, x, residual=None):
-        return ops.rms_norm(x, self.weight, self._eps(x), residual)
+        return ops.rms_norm(x, self.weight, self._eps(), residual)
 
 
 class SparseSequential(SparseModule):
@@ -172,7 +172,7 @@ class SparseSequential(SparseModule):
                     and ops.get_conv_math() == "f8" and i + 1 < len(mods)
                     and is_sparse_conv(mods[i + 1]) and mods[i + 1].pointwise):
                 x = input.features
-                f8, _ = ops.rms_norm_f8(x, module.weight, module._eps(x))
+                f8, _ = ops.rms_norm_f8(x, module.weight, module._eps())
                 n, bn, relu = self._fusable(mods, i + 1)
                 scale, shift = _bn_affine(bn) if bn is not None else (None, None)
                 input = mods[i + 1](input, _scale=scale, _shift=shift, _relu=relu, _f8=f8)

@@ -207,3 +207,25 @@ def _saved(module, file):
     torch.save(module, file)
     file.seek(0)
     return file
+
+
+@pytest.mark.parametrize("size", [1.0, 0.03, 0.001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rms_norm_module_without_eps_takes_that_of_float32(cuda, dtype, size):
+    """nn.RMSNorm's own default: the epsilon of the 32 bits that the norm is taken in, whatever the rows'
+    type (bf16 rows of RMS 0.03 under bf16's own epsilon of 2^-7 would come out a third as large)."""
+    x = (torch.randn((77, 96), generator=torch.Generator().manual_seed(7)) * size).to(dtype)
+    want, _, inv = ref.rms_norm(x, None, torch.finfo(torch.float32).eps)
+    # one store, and a chain of 96 squares, mean, root and division in fp32
+    bound = (ref.half_step(dtype) + 2.0 ** -24 * 120) * want.abs() + torch.finfo(dtype).tiny
+    y = spconv.RMSNorm(96).to(cuda)(x.to(cuda)).detach()
+    assert y.dtype == dtype and bool(((y.double().cpu() - want).abs() <= bound).all())
+    theirs = nn.RMSNorm(96, dtype=dtype)(x).detach().double()  # stored once as well
+    assert bool(((y.double().cpu() - theirs).abs() <= 2 * bound).all())
+    # straight to 8-bit rows, in front of a pointwise conv (values on a border of the format fall either way)
+    seq = spconv.SparseSequential(spconv.RMSNorm(96), spconv.SubMConv3d(96, 32, 1, bias=False)).to(cuda)
+    t = _tensor(cuda, 77, 96)
+    t.features = x.to(cuda)
+    with torch.no_grad(), ops.conv_math("f8"):
+        got = seq(t).features
+    _near(got, _q(want) @ _q(seq[1].weight.view(96, 32), 128), 2e-3 + ref.half_step(dtype))
