@@ -198,29 +198,33 @@ class SparseConvolution(SparseModule):
         """MFMA weight image (planes 2 / 3: the split bf16x3 / bf16x8 image; "f8": a pointwise conv's
         8-bit form), cached until the parameter is modified in place or replaced.  The cache holds the
         values that it was made from, so that their address stays theirs, and an event, for users on
-        another stream; an image made in a graph's capture is that graph's, and is not cached."""
+        another stream.  In a graph's capture the image is always made, whether one is cached or not:
+        it is then the graph's own memory, and replays follow the weight (a cached image would be freed
+        under the graph by the next call with a changed weight)."""
         w = self.weight
+        if torch.cuda.is_current_stream_capturing():
+            return self._make_weight_image(planes)
         tag = (w.data_ptr(), w._version, w.device, w.dtype)
         name = f"_wimg{planes}"
         cache = getattr(self, name, None)
         if cache is None or cache[0] != tag:
-            if planes == "f8":
-                img = ops.f8_weight_image(w.view(self.in_channels, self.out_channels),
-                                          transpose=True)
-            else:
-                img = ops.weight_image_bf16x3(w, planes=planes) if planes else ops.weight_image(w)
-            if torch.cuda.is_current_stream_capturing():
-                return img
+            img = self._make_weight_image(planes)
             maker = torch.cuda.current_stream(w.device)
             cache = (tag, img, w.detach(), maker, maker.record_event())
             object.__setattr__(self, name, cache)
         else:
             user = torch.cuda.current_stream(w.device)
-            if user != cache[3] and not torch.cuda.is_current_stream_capturing():
+            if user != cache[3]:
                 user.wait_event(cache[4])
                 for t in cache[1] if isinstance(cache[1], tuple) else (cache[1],):
                     t.record_stream(user)
         return cache[1]
+
+    def _make_weight_image(self, planes):
+        w = self.weight
+        if planes == "f8":
+            return ops.f8_weight_image(w.view(self.in_channels, self.out_channels), transpose=True)
+        return ops.weight_image_bf16x3(w, planes=planes) if planes else ops.weight_image(w)
 
 
 class SparseConv2d(SparseConvolution):

@@ -229,3 +229,47 @@ def test_rms_norm_module_without_eps_takes_that_of_float32(cuda, dtype, size):
     with torch.no_grad(), ops.conv_math("f8"):
         got = seq(t).features
     _near(got, _q(want) @ _q(seq[1].weight.view(96, 32), 128), 2e-3 + ref.half_step(dtype))
+
+
+@pytest.mark.parametrize("math", ["f8", "f32", "bf16x3"])
+def test_a_captured_graph_makes_its_own_weight_image(cuda, math):
+    """Warmed up, captured, then the weight changes and an ordinary call replaces the kept image: replays
+    follow the weight and read nothing that was freed."""
+    cin, cout, kernel = (256, 64, 1) if math == "f8" else (32, 32, 3)
+    conv = spconv.SubMConv3d(cin, cout, kernel, bias=False, indice_key="a").to(cuda)
+    x = _tensor(cuda, c=cin)
+    feats = x.features
+
+    def run():
+        x.features = feats
+        with torch.no_grad(), ops.conv_math(math):
+            return conv(x).features
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            run()
+    torch.cuda.current_stream().wait_stream(side)
+    before = run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, before)
+    for factor in (2.0, -0.5, 4.0):
+        with torch.no_grad():
+            conv.weight.mul_(factor)
+        scaled, before = before * factor, run()
+        # powers of two are exact in every mode; with the other sign the matrix cores may round a sum to
+        # its other neighbour (32 channels x 27 offsets x 3 products, 2^-23 each)
+        if factor > 0:
+            assert torch.equal(before, scaled)
+        assert float((before - scaled).abs().max()) <= 27 * 32 * 3 * 2.0 ** -23 * float(scaled.abs().max())
+        for _ in range(20):  # what was freed is somebody else's now
+            torch.full((cin * cout * kernel ** 3,), float("nan"), device=cuda)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, before) and torch.equal(run(), before)
