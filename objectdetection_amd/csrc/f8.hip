@@ -656,6 +656,9 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
     Rows x, y;
     ask(m0, x);
 
+    // Scale bytes of the blocks that there are.  Four steps serve three blocks too: the fourth is zeros,
+    // and what follows a row's scales is the caller's, 255 (no number) among it; made 0 it is 2^-127.
+    const unsigned scales = KS == 4 && p.K <= 384 ? 0xFFFFFFu : 0xFFFFFFFFu;
     f8_v8 fb[KS][4];
     unsigned xb[4];
     {
@@ -667,7 +670,7 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             const int n = min(f8_column<WIDE>(t, r16), p.N - 1 - n0);
-            xb[t] = *(const unsigned *)(p.sb + (long long)((n0 + n) >> p.b_shift) * p.ldsb);
+            xb[t] = *(const unsigned *)(p.sb + (long long)((n0 + n) >> p.b_shift) * p.ldsb) & scales;
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -711,7 +714,7 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
         int fa[KS][8];
         unsigned xa = 0;
         if constexpr (E == 1) {
-            xa = x.s;
+            xa = x.s & scales;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
 #pragma unroll

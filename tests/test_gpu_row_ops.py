@@ -762,3 +762,27 @@ def test_f8_linear_weight_gradient_of_strided_and_unfinished_rows(cuda, dtype):
     bad = torch.zeros((N, K), dtype=torch.bool, device=cuda)
     bad[:, 3] = bad[:, 17] = bad[9] = True
     assert bool(got[bad].isnan().all()) and bool(got[~bad].isfinite().all())
+
+
+@pytest.mark.parametrize("K", [300, 384])
+def test_f8_matmul_ignores_scales_behind_the_last_block(cuda, K):
+    """Scales that are the first columns of a wider matrix whose others mean nothing (255 is no number):
+    three blocks of 128, four bytes to a word."""
+    M, N = 4100, 72
+    a, b = _rows(80, M, K, torch.bfloat16), _rows(81, N, K, size=K ** -0.5)
+    xa, xb, w = ops.f8_rows(a.to(cuda)), ops.f8_rows(b.to(cuda)), ops.f8_weight_image(b.to(cuda))
+
+    def behind(x):
+        room = torch.full((x.scale.shape[0], 8), 255, dtype=torch.uint8, device=cuda)
+        room[:, :3] = x.scale.view(torch.uint8)
+        return ops.F8Rows(x.data, room[:, :3])
+    for out in DTYPES:
+        for m in (M, 3000, 40):  # rows past b in registers, tiles, few rows
+            part = ops.F8Rows(xa.data[:m], xa.scale[:m])
+            for image in (xb, w):
+                want = ops.f8_matmul(part, image, out_dtype=out)
+                assert bool(torch.isfinite(want).all())
+                for p, q in ((behind(part), image), (part, behind(image)), (behind(part), behind(image))):
+                    assert torch.equal(ops.f8_matmul(p, q, out_dtype=out), want), (out, m)
+    want = ops.f8_product(a.to(cuda), w)
+    assert torch.equal(ops.f8_product(a.to(cuda), behind(w)), want)
