@@ -390,6 +390,13 @@ void once(const char *who)
         fail(PyExc_RuntimeError, std::string(who) + " is differentiable once: no backward pass with create_graph=True");
 }
 bool wants(const Tensor *t) { return t && t->requires_grad(); }
+// a forward-mode tangent needs no requires_grad: the unrecorded path would drop it without a word
+void no_tangent(const char *who, std::initializer_list<const Tensor *> inputs)
+{
+    for (const Tensor *t : inputs)
+        if (t && t->_fw_grad(0).defined())
+            fail(PyExc_RuntimeError, std::string(who) + " has no forward-mode derivative");
+}
 
 struct Normed {
     Tensor y, h, inv;
@@ -616,6 +623,7 @@ PyObject *py_f8_linear(PyObject *, Args a, Py_ssize_t n)
         const Tensor &x = need(a[0]), &w = need(a[1]);
         const Tensor *bias = maybe(a[2]);
         const bool turned = truth(a[3]);
+        no_tangent("f8_linear", {&x, &w, bias});
         on_gpu(x);
         if (type_code(x.scalar_type()) < 0 || type_code(w.scalar_type()) < 0 || x.dim() != 2 || w.dim() != 2 ||
             x.size(1) != w.size(turned ? 0 : 1))
@@ -646,6 +654,7 @@ PyObject *py_rms_norm(PyObject *, Args a, Py_ssize_t n)
         const Tensor &x = need(a[0]);
         const Tensor *w = maybe(a[1]), *r = maybe(a[3]);
         const double eps = real(a[2]);
+        no_tangent("rms_norm", {&x, w, r});
         on_gpu(x);
         if (at::GradMode::is_enabled() && (wants(&x) || wants(w) || wants(r))) {
             const variable_list o = RmsNorm::apply(x, w ? Maybe(*w) : Maybe(), eps, r ? Maybe(*r) : Maybe());

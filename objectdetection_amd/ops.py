@@ -1304,8 +1304,8 @@ def rms_norm(x, weight=None, eps=1e-6, residual=None):
     float16; a row may start anywhere): y = h / sqrt(mean(h^2) + eps) * weight.  With ``residual``
     h = x + residual rounded to the rows' type, and (y, h) is returned; without it h = x and y is.
     Sums are held in 32 bits (a row whose squares sum past 3.4e38 comes out as zeros, as from the
-    formula in float32).  Differentiable once in x, weight and residual.  include/lcf.h:
-    lcf_rms_norm_fwd / _bwd."""
+    formula in float32).  Differentiable once, in reverse mode, in x, weight and residual (a forward-mode
+    tangent is refused).  include/lcf.h: lcf_rms_norm_fwd / _bwd."""
     return _lib.row_ops().rms_norm(x, weight, eps, residual)
 
 
@@ -1374,7 +1374,7 @@ def f8_linear(x, weight, bias=None, turned=False, x8=None):
     operands: -> [..., N] of x's type, differentiable in all three (weight and bias keep their own
     types): y, dx = dy W and dW = dy^T x are products of 8-bit operands whose scale blocks lie along
     the axis that the product sums over; the rounding is passed through unchanged.  Differentiable
-    once.  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.  K and N
+    once, in reverse mode (a forward-mode tangent is refused).  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.  K and N
     are 2^22 at most, and so are the rows where weight or bias wants a gradient.
     Error of an operand: half a step of e4m3, 2^-4 of a value, plus 2^-10 of its block's scale for
     small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""

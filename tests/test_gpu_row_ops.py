@@ -786,3 +786,20 @@ def test_f8_matmul_ignores_scales_behind_the_last_block(cuda, K):
                     assert torch.equal(ops.f8_matmul(p, q, out_dtype=out), want), (out, m)
     want = ops.f8_product(a.to(cuda), w)
     assert torch.equal(ops.f8_product(a.to(cuda), behind(w)), want)
+
+
+def test_forward_mode_derivatives_are_refused(cuda):
+    """A dual tensor need not require a gradient: without a refusal its tangent would be lost."""
+    from torch.autograd import forward_ad
+    x, w, r = (t.to(cuda) for t in (_rows(82, 20, 32), torch.ones(32), _rows(83, 20, 32)))
+    m, b = _rows(84, 8, 32).to(cuda), torch.zeros(8, device=cuda)
+    with forward_ad.dual_level():
+        for grad in (False, True):
+            def dual(t):
+                return forward_ad.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+            for call in (lambda: ops.rms_norm(dual(x), w), lambda: ops.rms_norm(x, dual(w)),
+                         lambda: ops.rms_norm(x, w, residual=dual(r)), lambda: ops.f8_linear(dual(x), m),
+                         lambda: ops.f8_linear(x, dual(m)), lambda: ops.f8_linear(x, m, dual(b))):
+                with pytest.raises(RuntimeError):
+                    call()
+        assert torch.equal(ops.rms_norm(x, w), ops.rms_norm(x.clone(), w))  # what has no tangent goes through

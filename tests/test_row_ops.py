@@ -151,3 +151,18 @@ def test_abi_refuses_bad_weight_gradients():
     assert grad(n=100) == WORKSPACE
     assert L.lcf_f8_weight_grad_workspace_bytes(100, 60, 32) == 0
     assert L.lcf_f8_weight_grad_workspace_bytes(100, 64, 32) >= (64 * 32 + 32) * 4
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor need not require a gradient, and nothing below autograd would carry its tangent."""
+    from torch.autograd import forward_ad
+    x, w = torch.ones((4, 8)), torch.ones((8,))
+    m, b = torch.ones((3, 8)), torch.ones((3,))
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.rms_norm(dual(x), w), lambda: ops.rms_norm(x, dual(w)),
+                     lambda: ops.rms_norm(x, w, residual=dual(x)), lambda: ops.f8_linear(dual(x), m),
+                     lambda: ops.f8_linear(x, dual(m)), lambda: ops.f8_linear(x, m, dual(b))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
