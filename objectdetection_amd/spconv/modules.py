@@ -23,6 +23,13 @@ def is_sparse_conv(module):
     return isinstance(module, SparseConvolution)
 
 
+def _plain(module, forward):
+    """``module`` does what ``forward`` does and nothing else: no forward of a subclass's or an
+    instance's own, no forward hooks."""
+    return (getattr(module.forward, "__func__", None) is forward
+            and not module._forward_hooks and not module._forward_pre_hooks)
+
+
 def _bn_affine(bn):
     """Eval-mode BatchNorm1d as y = x*scale + shift (fp32)."""
     inv = torch.rsqrt(bn.running_var.float() + bn.eps)
@@ -51,6 +58,12 @@ class RMSNorm(nn.RMSNorm):
         return ops.rms_norm(x, self.weight, self._eps(), residual)
 
 
+def _hands_over_8_bit_rows(norm, conv):
+    from .conv import SparseConvolution
+    return (is_sparse_conv(conv) and conv.pointwise and _plain(norm, RMSNorm.forward)
+            and _plain(conv, SparseConvolution.forward))
+
+
 class SparseSequential(SparseModule):
     """Sequential container that runs sparse modules on the SparseConvTensor and ordinary
     nn.Modules (BatchNorm1d, ReLU, ...) on its ``.features``.
@@ -62,7 +75,8 @@ class SparseSequential(SparseModule):
     ``BatchNorm1d (training) -> ReLU`` pair on the features runs as the fused streaming kernels of
     ``ops.bn_relu_train`` (same values and running statistics as the two torch modules;
     ``fuse_training = False`` to turn it off).  Under ``ops.conv_math("f8")`` without gradients an
-    ``RMSNorm -> pointwise sparse conv`` pair hands over 8-bit rows: the norm writes them itself.
+    ``RMSNorm -> pointwise sparse conv`` pair hands over 8-bit rows: the norm writes them itself (a
+    norm or conv with forward hooks, or of a subclass with its own forward, is called as a module).
     """
     fuse_inference = True
     fuse_training = True
@@ -170,7 +184,7 @@ class SparseSequential(SparseModule):
                     continue
             if (fuse and isinstance(module, RMSNorm) and isinstance(input, SparseConvTensor)
                     and ops.get_conv_math() == "f8" and i + 1 < len(mods)
-                    and is_sparse_conv(mods[i + 1]) and mods[i + 1].pointwise):
+                    and _hands_over_8_bit_rows(module, mods[i + 1])):
                 x = input.features
                 f8, _ = ops.rms_norm_f8(x, module.weight, module._eps())
                 n, bn, relu = self._fusable(mods, i + 1)

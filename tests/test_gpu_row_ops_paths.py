@@ -273,3 +273,49 @@ def test_a_captured_graph_makes_its_own_weight_image(cuda, math):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, before) and torch.equal(run(), before)
+
+
+class _Doubled(spconv.RMSNorm):
+    def forward(self, x, residual=None):
+        return 2 * super().forward(x, residual)
+
+
+class _Counted(spconv.SubMConv3d):
+    calls = 0
+
+    def forward(self, input):
+        _Counted.calls += 1
+        return super().forward(input)
+
+
+def test_norm_before_a_pointwise_conv_is_called_where_it_is_more_than_the_norm(cuda):
+    """A subclass's forward and forward hooks, of the norm or the conv, act under conv_math('f8') without
+    gradients as they do in every other mode."""
+    torch.manual_seed(8)
+    x = _tensor(cuda, 200, 64).features
+
+    def run(norm, conv):
+        t = _tensor(cuda, 200, 64)
+        with torch.no_grad(), ops.conv_math("f8"):
+            return spconv.SparseSequential(norm, conv)(t).features
+    conv = spconv.SubMConv3d(64, 32, 1, bias=False).to(cuda)
+    plain, twice = spconv.RMSNorm(64).to(cuda), _Doubled(64).to(cuda)
+    y = ref.rms_norm(x, None, torch.finfo(torch.float32).eps)[0]
+    w = _q(conv.weight.view(64, 32), 128)
+    _near(run(plain, conv), _q(y) @ w, 2e-3)
+    _near(run(twice, conv), _q(2 * y) @ w, 2e-3)
+    seen = []
+    plain.register_forward_pre_hook(lambda m, args: seen.append(args[0].shape))
+    _near(run(plain, conv), _q(y) @ w, 2e-3)
+    assert seen == [(200, 64)]
+    hooked = spconv.RMSNorm(64).to(cuda)
+    hooked.register_forward_hook(lambda m, args, out: out * 4)
+    _near(run(hooked, conv), _q(4 * y) @ w, 2e-3)
+    own = _Counted(64, 32, 1, bias=False).to(cuda)
+    own.load_state_dict(conv.state_dict())
+    _near(run(spconv.RMSNorm(64).to(cuda), own), _q(y) @ w, 2e-3)
+    assert _Counted.calls == 1
+    rows = []
+    conv.register_forward_pre_hook(lambda m, args: rows.append(args[0].features))
+    _near(run(spconv.RMSNorm(64).to(cuda), conv), _q(y) @ w, 2e-3)
+    _near(rows[0], y, 1e-6)  # the normed rows, not those in front of the norm
