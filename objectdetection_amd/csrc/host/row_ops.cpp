@@ -502,17 +502,17 @@ Tensor f8_linear_fwd(const Tensor &x, const Tensor &w, const Tensor *bias, bool 
     return f8_mm(*x8, image, nullptr, sh, false, type_code(x.scalar_type()), nullptr, on.st);
 }
 
-// dw and, with bias >= 0, db of that type, where lcf_f8_weight_grad takes the sizes; false elsewhere
-bool f8_weight_grad(const Tensor &x, const Tensor &dy, bool turned, const Tensor &w, int bias, Tensor &dw, Tensor &db, void *st)
+// dw of type code w and, with bias >= 0, db of that type, where lcf_f8_weight_grad takes the sizes; false elsewhere
+bool f8_weight_grad(const Tensor &x, const Tensor &dy, bool turned, int w, int bias, Tensor &dw, Tensor &db, void *st)
 {
     const int R = count(x.size(0), "f8_linear"), K = count(x.size(1), "f8_linear"), N = count(dy.size(1), "f8_linear");
     const size_t n = L.f8_weight_grad_workspace_bytes(R, K, N);
     if (!n) return false;
     const Rows xv = rows_of(x, K), dv = rows_of(dy, N);
-    const Tensor ws = bytes(n, x), to = at::empty(w.sizes(), w.options()),
+    const Tensor ws = bytes(n, x), to = at::empty({turned ? K : N, turned ? N : K}, x.options().dtype(type_of(w))),
                  sum = bias >= 0 ? at::empty({N}, x.options().dtype(type_of(bias))) : Tensor();
     const int rc = L.f8_weight_grad(xv.ptr(), xv.ld, dv.ptr(), dv.ld, R, K, N, type_code(x.scalar_type()), turned,
-                                    to.data_ptr(), type_code(w.scalar_type()), bias >= 0 ? sum.data_ptr() : nullptr,
+                                    to.data_ptr(), w, bias >= 0 ? sum.data_ptr() : nullptr,
                                     bias >= 0 ? bias : 0, ws.data_ptr(), (size_t)ws.numel(), st);
     if (rc == LCF_ERR_UNSUPPORTED) return false;
     check(rc);
@@ -530,8 +530,12 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
     {
         F8 back;
         Tensor y = f8_linear_fwd(x, w, maybe(bias), turned, x8, x.requires_grad() ? &back : nullptr);
-        ctx->save_for_backward({x, w, back.data, back.scale});
+        // the rows are for the weight's gradient alone, and of the weight its type is enough: what is not kept
+        // costs no memory and may be written to
+        ctx->save_for_backward({w.requires_grad() ? x : Tensor(), back.data, back.scale});
         ctx->saved_data["turned"] = turned;
+        ctx->saved_data["x"] = (int64_t)type_code(x.scalar_type());
+        ctx->saved_data["w"] = (int64_t)type_code(w.scalar_type());
         ctx->saved_data["bias"] = (int64_t)(maybe(bias) ? type_code(bias->scalar_type()) : -1);
         return y;
     }
@@ -540,19 +544,20 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
         once("f8_linear");
         at::AutoDispatchBelowADInplaceOrView below;
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &w = saved[1];
+        const Tensor &x = saved[0];
         const bool turned = ctx->saved_data["turned"].toBool();
-        const int bias = (int)ctx->saved_data["bias"].toInt();
+        const int w = (int)ctx->saved_data["w"].toInt(), bias = (int)ctx->saved_data["bias"].toInt();
         const bool need_x = ctx->needs_input_grad(0);
         bool need_w = ctx->needs_input_grad(1), need_b = bias >= 0 && ctx->needs_input_grad(2);
-        const On on(x);
         Tensor dy = grads[0], dx, dw, db;
-        if (dy.scalar_type() != x.scalar_type()) dy = dy.to(x.scalar_type());
+        const On on(dy);
+        const at::ScalarType rows_type = type_of((int)ctx->saved_data["x"].toInt());
+        if (dy.scalar_type() != rows_type) dy = dy.to(rows_type);
         // the input's gradient takes dy as it is where one launch does both; elsewhere dy's rows form, its
         // columns form and the bias's sums come out of one reading
         F8 image;
         if (need_x) {
-            image = f8_operand(saved[2], saved[3], "weight");
+            image = f8_operand(saved[1], saved[2], "weight");
             dx = f8_fused(dy, image, nullptr, nullptr, false, on.st);
         }
         // the weight's gradient and the bias's take both as they are where one kernel does all
@@ -566,8 +571,7 @@ struct F8Linear : torch::autograd::Function<F8Linear> {
         if (rows) dx = f8_mm(q.rows, image, nullptr, nullptr, false, type_code(dy.scalar_type()), nullptr, on.st);
         if (need_w) {
             const F8 xt = f8_quant(x, LCF_E4M3, false, false, true, false, on.st).cols;
-            dw = f8_mm(turned ? xt : q.cols, turned ? q.cols : xt, nullptr, nullptr, false, type_code(w.scalar_type()),
-                       nullptr, on.st);
+            dw = f8_mm(turned ? xt : q.cols, turned ? q.cols : xt, nullptr, nullptr, false, w, nullptr, on.st);
         }
         if (need_b) {
             const int C = (int)dy.size(1);

@@ -803,3 +803,34 @@ def test_forward_mode_derivatives_are_refused(cuda):
                 with pytest.raises(RuntimeError):
                     call()
         assert torch.equal(ops.rms_norm(x, w), ops.rms_norm(x.clone(), w))  # what has no tangent goes through
+
+
+def test_f8_linear_keeps_only_what_its_gradients_take(cuda):
+    """The rows are kept for the weight's gradient alone and the weight not at all: a layer whose weight
+    is frozen does not mind its rows being written to, nor a first layer its weight being stepped."""
+    x0, w0, b0 = _rows(85, 50, 48).to(cuda), _rows(86, 24, 48).to(cuda), torch.zeros(24, device=cuda)
+    dy = _rows(87, 50, 24).to(cuda)
+
+    def grads(frozen, first, late):
+        x, w, b = x0.clone(), w0.clone(), b0.clone().requires_grad_(True)
+        leaf = x0.clone().requires_grad_(not first)
+        w.requires_grad_(not frozen)
+        rows = leaf * 1.0 if not first else x
+        y = ops.f8_linear(rows, w, b)
+        with torch.no_grad():
+            if late and frozen:
+                rows.zero_()
+            if late:
+                w.zero_()
+        y.backward(dy)
+        return [t.grad for t in (leaf, w, b) if t.requires_grad]
+    for frozen, first in ((True, False), (False, True), (True, True), (False, False)):
+        want, got = grads(frozen, first, False), grads(frozen, first, True)
+        assert len(got) == 3 - frozen - first
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+    # rows that the weight's gradient does take may not change in between
+    x, w = x0.clone(), w0.clone().requires_grad_(True)
+    y = ops.f8_linear(x, w)
+    x.zero_()
+    with pytest.raises(RuntimeError):
+        y.backward(dy)
