@@ -1380,5 +1380,6 @@ def f8_linear(x, weight, bias=None, turned=False, x8=None):
     small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
     if x.dim() == 2:
         return _lib.row_ops().f8_linear(x, weight, bias, turned, x8)
-    y = _lib.row_ops().f8_linear(x.reshape(-1, x.shape[-1]), weight, bias, turned, x8)
+    rows = x.flatten(0, -2) if x.dim() > 2 else x.unsqueeze(0)  # (-1 is ambiguous where K = 0)
+    y = _lib.row_ops().f8_linear(rows, weight, bias, turned, x8)
     return y.view(*x.shape[:-1], y.shape[1])

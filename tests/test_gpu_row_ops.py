@@ -834,3 +834,17 @@ def test_f8_linear_keeps_only_what_its_gradients_take(cuda):
     x.zero_()
     with pytest.raises(RuntimeError):
         y.backward(dy)
+
+
+@pytest.mark.parametrize("lead", [(2, 3), (0, 3), (), (4,)])
+def test_f8_linear_of_no_columns_and_of_any_leading_sizes(cuda, lead):
+    bias = torch.randn((8,), generator=_gen(88)).to(cuda)
+    for K in (0, 32):
+        x = torch.randn((*lead, K), generator=_gen(89)).to(cuda).requires_grad_(True)
+        w = torch.randn((8, K), generator=_gen(90)).to(cuda).requires_grad_(True)
+        y = ops.f8_linear(x, w, bias)
+        assert y.shape == (*lead, 8)
+        rows = ops.f8_linear(x.detach().reshape(math.prod(lead), K), w.detach(), bias)
+        assert torch.equal(y.detach().reshape(math.prod(lead), 8), rows)
+        y.sum().backward()
+        assert x.grad.shape == x.shape and w.grad.shape == w.shape
