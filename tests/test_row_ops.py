@@ -166,3 +166,20 @@ def test_forward_mode_tangents_are_refused():
                      lambda: ops.f8_linear(x, dual(m)), lambda: ops.f8_linear(x, m, dual(b))):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def test_a_change_of_the_build_flags_rebuilds_every_object():
+    """Objects are ignored by git and outlive a change of the Makefile's flags: one that keeps the packed
+    fp32 instructions would go unnoticed."""
+    import os
+    import re
+    import subprocess
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    plan = subprocess.run(["make", "-n", "-W", "Makefile", "-C", csrc], capture_output=True, text=True, check=True).stdout
+    sources = re.search(r"^SRCS := ((?:.*\\\n)*.*)$", open(os.path.join(csrc, "Makefile")).read(), re.M).group(1)
+    sources = sources.replace("\\", " ").split()
+    assert len(sources) >= 12
+    for source in sources:
+        line = next(k for k in plan.splitlines() if f"-c {source} " in k)
+        assert "-packed-fp32-ops" in line
+    assert "-o ../_row_ops.so" in plan and "-o ../liblcf_cpu.so" in plan and "-o ../liblcf.so" in plan
