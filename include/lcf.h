@@ -769,9 +769,11 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  *   magnitudes; about 1.5e-5 of the result on random data), then one rounding.
  *   K == 0 gives act(shift).  LCF_ERR_UNSUPPORTED: lda or ldb > 2^22, M or N > 2^31 - 256, N > 2^25
  *   where M <= 64, 2^23 tiles of the output or more (the smallest are of 64 x 128 and 128 x 64).
- *   ws: lcf_f8_gemm_workspace_bytes(M, N, K, out_dtype) (0 for most sizes: the sum is split over
- *   workgroups only where the output has few tiles; the parts are joined in a fixed order, so
- *   results are run-to-run identical). */
+ *   ws: lcf_f8_gemm_workspace_bytes(M, N, K, out_dtype) (0 for most sizes, M <= 64 among them: the sum is
+ *   split over workgroups only where the output has few tiles; the parts are joined in a fixed order, so
+ *   results are run-to-run identical).  With lcf_f8_gemm_split_bytes of it, which is never less, the long
+ *   sums of few rows are split as well (M <= 64; many times as fast: 50 x 200 over K = 136000 19 us
+ *   instead of 226); the order of a sum, and so its last bits, go by whether it is split. */
 int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtype, int fmt, int square, void *q,
                  long long ldq, unsigned char *s, int lds, void *qt, long long ldqt,
                  unsigned char *st, int ldst, float *sums, void *stream);
@@ -779,6 +781,7 @@ int lcf_f8_quant(const void *x, long long ldx, int R, int C, int dtype, int fmt,
  * (LCF_ERR_UNSUPPORTED). */
 int lcf_sum_parts(const float *parts, int count, int n, void *out, int dtype, void *stream);
 size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype);
+size_t lcf_f8_gemm_split_bytes(int M, int N, int K, int out_dtype);
 int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa, int ldsa, int a_fmt,
                 const void *b, long long ldb, const unsigned char *sb, int ldsb, int b_fmt,
                 int b_square, int M, int N, int K, const float *scale, const float *shift, int relu,

@@ -206,6 +206,7 @@ SYMBOLS = {
                              c_void_p]),
     "lcf_sum_parts": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
     "lcf_f8_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "lcf_f8_gemm_split_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "lcf_f8_linear": (c_int, [c_void_p, c_ll, c_int, c_void_p, c_ll, c_void_p, c_int, c_int, c_int,
                               c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_ll, c_int,
                               c_void_p]),

@@ -849,8 +849,8 @@ __global__ void __launch_bounds__(256) f8_stream_kernel(F8Gemm p, int wn_shift)
     }
 }
 
-// A few rows (M <= 64): bound by reading b once.  A workgroup takes 16 columns of the output, its waves
-// take turns of 512 bytes along k (four steps, one scale word): everything of a turn is asked for at
+// A few rows (M <= 64, unless their sums are long and split: f8_long): bound by reading b once.  A
+// workgroup takes 16 columns of the output, its waves take turns of 512 bytes along k (four steps, one scale word): everything of a turn is asked for at
 // once, 8 KB of b a wave, straight into registers.  The waves' sums meet in LDS in a fixed order.
 // (Tiles of 128 rows leave a compute unit one 16 KB step in flight: 11.6 us and a join of 3.9 us at
 // 8 x 8192 x 4096; now 12.4 us, 2.7 TB/s with the launch and the first latency in it.)
@@ -1002,16 +1002,28 @@ enum { F8_256, F8_128, F8_64, F8_NARROW };
 struct F8Plan {
     int thin, few, shape, tiles_m, tiles_n, splits, ksteps;
 };
-static F8Plan f8_plan(int M, int N, int K, bool wide)
+// A few rows over a long sum: f8_few_kernel has a workgroup for 16 columns walk all of k, and every piece
+// of 16 rows adds to a turn, where the tiles divide k over the chip.  The border, us of f8_few_kernel and of
+// the tiles with their split: 8 x 1024 columns, K 4096 6.4 / 8.5, 8192 9.7 / 8.6, 16384 16.6 / 9.3, 131072
+// 107 / 31; 64 x 1024 columns, K 2048 8.3 / 9.3, 4096 13.4 / 9.9, 131072 328 / 34; 50 x 200 over 136000 rows
+// (a weight gradient) 226 / 19.  Up to 16 rows more than 8192 columns are workgroups enough by themselves
+// (8 x 16384, K 16384 63 / 100; 8 x 8192 38 / 30, and past 256 MB of b 121 / 141, left to the tiles).
+static bool f8_long(int M, int N, int K)
+{
+    const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    return (long long)mt * K > 8192 && (M > 16 || N <= 8192);
+}
+// divided: whether there is a workspace for dividing the sums of a few rows
+static F8Plan f8_plan(int M, int N, int K, bool wide, bool divided)
 {
     F8Plan q;
     q.thin = f8_is_thin(M, N, K, wide);
-    q.few = M <= 64 && K > 0;
+    q.few = M <= 64 && K > 0 && !(divided && f8_long(M, N, K));
     const long long t256 = (long long)((M + 255) / 256) * ((N + 255) / 256);
     const long long t128 = (long long)((M + 127) / 128) * ((N + 127) / 128);
     // the largest tile that still gives the 256 units work: 256 x 256 (one workgroup fills a unit),
     // 128 x 128 (two do), 64 x 128 (three do); 128 x 64 where there are no more columns
-    q.shape = N <= 64 ? F8_NARROW : t256 >= 192 ? F8_256 : t128 >= 512 ? F8_128 : F8_64;
+    q.shape = N <= 64 ? F8_NARROW : M <= 64 ? F8_64 : t256 >= 192 ? F8_256 : t128 >= 512 ? F8_128 : F8_64;
     const int bm = q.shape == F8_256 ? 256 : q.shape == F8_64 ? 64 : 128;
     const int bn = q.shape == F8_256 ? 256 : q.shape == F8_NARROW ? 64 : 128;
     q.tiles_m = (M + bm - 1) / bm;
@@ -1032,11 +1044,18 @@ static F8Plan f8_plan(int M, int N, int K, bool wide)
     return q;
 }
 
-extern "C" size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype)
+static size_t f8_parts_bytes(const F8Plan &q, int M, int N)
+{
+    return q.splits > 1 ? (size_t)q.splits * M * N * sizeof(float) : 0;
+}
+extern "C" size_t lcf_f8_gemm_split_bytes(int M, int N, int K, int out_dtype)
 {
     if (M < 1 || N < 1 || K < 1 || M > F8_MOST || N > F8_MOST || K > F8_MOST) return 0;
-    const F8Plan q = f8_plan(M, N, K, out_dtype == LCF_F32);
-    return q.splits > 1 ? (size_t)q.splits * M * N * sizeof(float) : 0;
+    return f8_parts_bytes(f8_plan(M, N, K, out_dtype == LCF_F32, true), M, N);
+}
+extern "C" size_t lcf_f8_gemm_workspace_bytes(int M, int N, int K, int out_dtype)
+{
+    return M <= 64 ? 0 : lcf_f8_gemm_split_bytes(M, N, K, out_dtype);
 }
 
 // whether f8_stream_kernel takes a product: b in registers, rows enough for every wave, and whole
@@ -1161,13 +1180,15 @@ extern "C" int lcf_f8_gemm(const void *a, long long lda, const unsigned char *sa
     // a tile's rows are addressed in 32 bits, and a launch has fewer than 2^32 threads (512 a tile at
     // most, 1024 for 16 columns of a few rows)
     if (lda > (1 << 22) || ldb > (1 << 22) || M > F8_MOST || N > F8_MOST) return LCF_ERR_UNSUPPORTED;
-    const F8Plan q = f8_plan(M, N, K, out_dtype == LCF_F32);
+    F8Plan q = f8_plan(M, N, K, out_dtype == LCF_F32, true);
+    if (M <= 64 && q.splits > 1 && (!ws || ws_bytes < f8_parts_bytes(q, M, N)))
+        q = f8_plan(M, N, K, out_dtype == LCF_F32, false);
     const bool thin = q.thin && f8_out_ok(out, ldo, out_dtype);
-    if (!thin && (q.few ? N > 1 << 25 : (long long)q.tiles_m * q.tiles_n * q.splits > (1 << 23) - 8))
+    if (!thin && (M <= 64 && K > 0 ? N > 1 << 25 : (long long)q.tiles_m * q.tiles_n * q.splits > (1 << 23) - 8))
         return LCF_ERR_UNSUPPORTED;
     if (q.splits > 1) {
         if (!ws) return LCF_ERR_ARG;
-        if (ws_bytes < (size_t)q.splits * M * N * sizeof(float)) return LCF_ERR_WORKSPACE;
+        if (ws_bytes < f8_parts_bytes(q, M, N)) return LCF_ERR_WORKSPACE;
     }
     F8Gemm p{(const unsigned char *)a, sa, (const unsigned char *)b, sb, scale, shift, out,
              q.splits > 1 ? (float *)ws : nullptr, lda, ldb, ldo, ldsa, ldsb, b_square ? 7 : 0, M, N, K, relu,

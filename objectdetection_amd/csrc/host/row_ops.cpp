@@ -29,7 +29,7 @@ struct Err : std::runtime_error {
 
 #define LCF_FUNCTIONS(F)                                                                                       \
     F(strerror) F(grad_norm_workspace_bytes) F(grad_norm) F(grad_clip) F(rms_norm_fwd) F(rms_norm_workspace_bytes) \
-    F(rms_norm_bwd) F(f8_quant) F(f8_gemm_workspace_bytes) F(f8_gemm) F(f8_linear) F(sum_parts) \
+    F(rms_norm_bwd) F(f8_quant) F(f8_gemm_split_bytes) F(f8_gemm) F(f8_linear) F(sum_parts) \
     F(f8_weight_grad_workspace_bytes) F(f8_weight_grad)
 struct Lib {
 #define F(name) decltype(&lcf_##name) name;
@@ -288,7 +288,7 @@ at::Tensor f8_mm(const F8 &a, const F8 &b, const at::Tensor *scale, const at::Te
         if (code < 0) fail(PyExc_TypeError, "f8_matmul: out_dtype must be float32, bfloat16 or float16");
         out = at::empty({M, N}, a.data.options().dtype(type_of(code)));
     }
-    const size_t n = L.f8_gemm_workspace_bytes(M, N, K, code);
+    const size_t n = L.f8_gemm_split_bytes(M, N, K, code);
     at::Tensor ws;
     if (n) ws = bytes(n, a.data);
     if (to) written(out);

@@ -848,3 +848,47 @@ def test_f8_linear_of_no_columns_and_of_any_leading_sizes(cuda, lead):
         assert torch.equal(y.detach().reshape(math.prod(lead), 8), rows)
         y.sum().backward()
         assert x.grad.shape == x.shape and w.grad.shape == w.shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(50, 200, 20011), (64, 260, 9000), (17, 65, 8200), (1, 16, 30000), (16, 129, 8193),
+                                   (33, 24, 4100), (48, 1000, 5000)])
+def test_f8_matmul_long_sums_of_few_rows(cuda, shape, dtype):
+    """Few rows over a long sum, split over workgroups, and the same call into the library without room for
+    the split."""
+    M, N, K = shape
+    L, code = ops._lib.lib(), ops._TYPE_CODE[dtype]
+    assert L.lcf_f8_gemm_split_bytes(M, N, K, code) > L.lcf_f8_gemm_workspace_bytes(M, N, K, code) == 0
+    a, b = _rows(91, M, K), _rows(92, N, K, size=K ** -0.5)
+    scale, shift = torch.rand((N,), generator=_gen(93)) + 0.5, torch.randn((N,), generator=_gen(94))
+    qa, qb = ref.value(*ref.quantise(a)), ref.value(*ref.quantise(b))
+    y = qa @ qb.t()
+    xa, xb = ops.f8_rows(a.to(cuda)), ops.f8_rows(b.to(cuda))
+    s, t = scale.to(cuda), shift.to(cuda)
+    got = [ops.f8_matmul(xa, xb, s, t, True, dtype) for _ in range(3)]
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    one = torch.empty((M, N), dtype=dtype, device=cuda)
+    assert L.lcf_f8_gemm(xa.data.data_ptr(), xa.data.stride(0), xa.scale.data_ptr(), xa.scale.stride(0), 0,
+                         xb.data.data_ptr(), xb.data.stride(0), xb.scale.data_ptr(), xb.scale.stride(0), 0, 0, M, N, K,
+                         s.data_ptr(), t.data_ptr(), 1, one.data_ptr(), N, code, None, 0,
+                         torch.cuda.current_stream().cuda_stream) == 0
+    want = (y * scale.double() + shift.double()).clamp(min=0)
+    bound = (scale.double() * _product_bound(qa, qb, K, y, dtype)
+             + 4 * F32 * (y.abs() * scale.double() + shift.double().abs()) + half_step(dtype) * want * 1.01 + tiny(dtype))
+    _within(got[0], want, bound, "split")
+    _within(one, want, bound, "whole")
+
+
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("shape", [(20000, 50, 200), (9001, 260, 64), (30000, 18, 33)])
+def test_f8_linear_weight_gradients_of_few_channels(cuda, shape, turned):
+    """Channel counts that are no multiples of 8, or more than 256, over many rows."""
+    M, N, K = shape
+    x = _rows(95, M, K, torch.bfloat16).to(cuda)
+    w = _rows(96, N, K, size=K ** -0.5).to(cuda)
+    leaf = (w.t().contiguous() if turned else w).requires_grad_(True)
+    dy = _rows(97, M, N, torch.bfloat16, 1e-2)
+    dw, = torch.autograd.grad(ops.f8_linear(x, leaf, turned=turned), leaf, dy.to(cuda))
+    dt, xt = ref.value(*ref.quantise(dy.t())), ref.value(*ref.quantise(x.t()))
+    want = dt @ xt.t()
+    _within(dw.t() if turned else dw, want, _product_bound(dt, xt, M, want, torch.float32), "dw")

@@ -183,3 +183,21 @@ def test_a_change_of_the_build_flags_rebuilds_every_object():
         line = next(k for k in plan.splitlines() if f"-c {source} " in k)
         assert "-packed-fp32-ops" in line
     assert "-o ../_row_ops.so" in plan and "-o ../liblcf_cpu.so" in plan and "-o ../liblcf.so" in plan
+
+
+def test_long_sums_of_few_rows_are_split_where_there_is_room():
+    """A weight gradient of few channels is few rows over a long sum: without a split 13 workgroups walk
+    all of it.  The room is offered, not asked for."""
+    L = _lib.lib()
+    for M, N, K in ((50, 200, 136000), (64, 512, 136000), (18, 128, 136000), (64, 260, 136000), (8, 16, 90000),
+                    (40, 64, 70000), (17, 1000, 8192), (33, 24, 4096), (16, 8192, 8193)):
+        for t in range(3):
+            assert L.lcf_f8_gemm_workspace_bytes(M, N, K, t) == 0
+            parts, rest = divmod(L.lcf_f8_gemm_split_bytes(M, N, K, t), M * N * 4)
+            assert rest == 0 and 2 <= parts <= 256, (M, N, K, t, parts)
+    for M, N, K in ((8, 8192, 4096), (1, 4096, 8192), (64, 256, 2048), (32, 64, 4096), (16, 8200, 30000)):
+        assert L.lcf_f8_gemm_split_bytes(M, N, K, 0) == 0
+    for M, N, K in ((65, 200, 136000), (100, 64, 9000), (8192, 4096, 8192)):  # many rows need what they are offered
+        assert L.lcf_f8_gemm_split_bytes(M, N, K, 0) == L.lcf_f8_gemm_workspace_bytes(M, N, K, 0)
+    last = (1 << 31) - 1
+    assert L.lcf_f8_gemm_split_bytes(last, last, 64, 0) == 0 and L.lcf_f8_gemm_split_bytes(0, 5, 64, 0) == 0
