@@ -764,7 +764,9 @@ int lcf_rms_norm_bwd(const void *h, long long ldh, const void *dy, long long ldd
  *   form, b_square != 0: b has 128 x 128 scale blocks; scale / shift fp32 or NULL, relu != 0 clamps
  *   at 0; out [M, N] of out_dtype, ldo elements between rows.  What lies in a row behind column K
  *   does not enter.  out_dtype fp32: exact products summed in fp32 (bytes widened to bf16 in
- *   registers); bf16 / fp16: the 8-bit matrix instructions, whose sums of eight neighbouring
+ *   registers, which is exact but at the ends of the range: values below 2^-126 become the nearest multiple
+ *   of 2^-133 -- in blocks of e < -124 (e4m3) or -117 (e5m2) only -- and those of 2^128 and more
+ *   infinite); bf16 / fp16: the 8-bit matrix instructions, whose sums of eight neighbouring
  *   products keep 13 bits below the largest of them (an error of at most 2^-10 of the sum of
  *   magnitudes; about 1.5e-5 of the result on random data), then one rounding.
  *   K == 0 gives act(shift).  LCF_ERR_UNSUPPORTED: lda or ldb > 2^22, M or N > 2^31 - 256, N > 2^25

@@ -13,7 +13,8 @@
 //     2^-10 of a group's sum of magnitudes, and 1.5e-5 of the result on random data -- a 16-bit store
 //     rounds by up to 2^-8 (bf16) or 2^-11 (fp16) of it.  Not what an fp32 output promises.
 //   fp32 outputs: the bytes become bf16 in registers, scaled (v_cvt_scalef32_pk_bf16_*: q 2^e is
-//     exact), and v_mfma_f32_16x16x32_bf16 adds the exact products in fp32, at half the peak rate.
+//     exact, but below 2^-126, where it is rounded to a multiple of 2^-133, and from 2^128 on, where it is
+//     infinite), and v_mfma_f32_16x16x32_bf16 adds the exact products in fp32, at half the peak rate.
 #include "rows.h"
 
 typedef int f8_v8 __attribute__((ext_vector_type(8)));

@@ -98,7 +98,10 @@ __device__ __forceinline__ void lcf_ld8_code(const void *p, int code, int col, i
 // 1.75 * 2^8 (e4m3) or 1.75 * 2^15 (e5m2), so with amax = m * 2^x, 1 <= m < 2, e is x - 8 (x - 15),
 // and one more when m > 1.75.  e is held in [-126, 127] and stored as the E8M0 byte e + 127: the
 // scaled MFMA takes that byte as an operand, so scales cost a product no vector instruction, and
-// q * 2^e is exact in fp32 and in bf16.  A block of zeros has e = 0.
+// q * 2^e is exact in fp32 and, from e = -124 (e4m3) or -117 (e5m2) on, in bf16: below, the format's least
+// values are no bf16 numbers and round to a multiple of 2^-133, bf16's least step.  (At the other end a
+// block whose largest magnitude rounds up to 2^128 stands for a number that neither type holds.)  A block
+// of zeros has e = 0.
 __device__ __forceinline__ int lcf_f8_exponent(float amax, int fmt)
 {
     const unsigned u = __float_as_uint(amax);

@@ -892,3 +892,32 @@ def test_f8_linear_weight_gradients_of_few_channels(cuda, shape, turned):
     dt, xt = ref.value(*ref.quantise(dy.t())), ref.value(*ref.quantise(x.t()))
     want = dt @ xt.t()
     _within(dw.t() if turned else dw, want, _product_bound(dt, xt, M, want, torch.float32), "dw")
+
+
+@pytest.mark.parametrize("shape", [(8, 24, 130), (100, 64, 300), (4100, 16, 128)])
+@pytest.mark.parametrize("f8", [E4M3, E5M2])
+def test_f8_matmul_at_the_ends_of_the_scales(cuda, f8, shape):
+    """Blocks of the smallest scale against blocks of large ones: fp32 outputs widen to bf16, whose least
+    step is 2^-133 (half of it for each element, times what it meets); the 8-bit instruction has no such end."""
+    M, N, K = shape
+    size = torch.exp(-8 * torch.rand((M, 1), generator=_gen(98)))  # magnitudes from 1e-35 down to 1e-38 and less
+    a = _rows(99, M, K) * size * 1e-35
+    a[0] = a[0] * 1e-5
+    b = _rows(100, N, K) * 1e35
+    for left, right, swap in ((a, b, False), (b, a, True)):
+        qa, qb = ref.value(*ref.quantise(left, f8)), ref.value(*ref.quantise(right, f8))
+        want = qa @ qb.t()
+        xa, xb = ops.f8_rows(left.to(cuda), f8), ops.f8_rows(right.to(cuda), f8)
+        rounded = 2.0 ** -134 * (qb.abs().sum(1)[None, :] if not swap else qa.abs().sum(1)[:, None])
+        for out in (torch.float32, torch.bfloat16):
+            got = ops.f8_matmul(xa, xb, out_dtype=out)
+            bound = _product_bound(qa, qb, K, want, out) + (1 + 2 * K * F32) * (rounded if out == torch.float32 else 0.0)
+            _within(got, want, bound, (out, swap))
+    # a block whose largest magnitude rounds up to 2^128
+    top = torch.zeros((M, 128))
+    top[:, 0] = 3.4e38
+    one = torch.zeros((N, 128))
+    one[:, 0] = 2.0 ** -40
+    xa, xb = ops.f8_rows(top.to(cuda)), ops.f8_rows(one.to(cuda))
+    assert bool((ops.f8_matmul(xa, xb) == float("inf")).all())
+    assert bool((ops.f8_matmul(xa, xb, out_dtype=torch.bfloat16) == 2.0 ** 88).all())
