@@ -1321,7 +1321,8 @@ def rms_norm_f8(x, weight=None, eps=1e-6, residual=None, dtype=torch.float8_e4m3
 
 # A matrix [R, C] in 8-bit form: data [R, C] float8 and scale float8_e8m0fnu, [R, ceil(C / 128)]
 # (one power of two for each 128 columns of a row) or [ceil(R / 128), ceil(C / 128)] (for each
-# 128 x 128: weights).  An element stands for data * scale.  Rows of data start on 16-byte borders
+# 128 x 128: weights).  None of the functions below but f8_linear is recorded by autograd: what they
+# return has no gradient, also where an operand, scale or shift requires one.  An element stands for data * scale.  Rows of data start on 16-byte borders
 # and rows of scale on 4-byte borders (the views that the functions below return have such strides).
 F8Rows = namedtuple("F8Rows", ["data", "scale"])
 
@@ -1330,7 +1331,7 @@ def f8_rows(x, dtype=torch.float8_e4m3fn):
     """x [R, C] (float32, bfloat16 or float16) in 8-bit form, blocks of 128 along each row (what a
     product over C takes): q = round(x * 2^-e) to nearest even, 2^e the smallest power of two that
     brings the block's largest finite magnitude inside the format; infinities and NaN become NaN.
-    include/lcf.h: lcf_f8_quant."""
+    No gradient flows through it.  include/lcf.h: lcf_f8_quant."""
     return F8Rows(*_lib.row_ops().f8_rows(x, _f8_code(dtype)))
 
 
@@ -1359,13 +1360,13 @@ def f8_matmul(a, b, scale=None, shift=None, relu=False, out_dtype=torch.float32,
     float32 or None, act = max(x, 0) with ``relu``; out_dtype float32, bfloat16 or float16 (the
     arithmetic goes by it, see include/lcf.h: lcf_f8_gemm).  Rows that do not start on the borders
     the kernels read from are copied once.  ``out``: caller-owned [M, N] with unit stride in a
-    row."""
+    row.  No gradient flows through it, nor to scale and shift (``f8_linear`` has them)."""
     return _lib.row_ops().f8_mm(a, b, scale, shift, relu, _TYPE_CODE.get(out_dtype, -1), out)
 
 
 def f8_product(x, b, scale=None, shift=None, relu=False):
     """f8_matmul(f8_rows(x), b, ...) of x's own type: one launch where lcf_f8_linear takes the sizes
-    (thin layers over many rows; the same bits), two elsewhere."""
+    (thin layers over many rows; the same bits), two elsewhere.  No gradient flows through it."""
     return _lib.row_ops().f8_product(x, b, scale, shift, relu)
 
 
@@ -1377,7 +1378,10 @@ def f8_linear(x, weight, bias=None, turned=False, x8=None):
     once, in reverse mode (a forward-mode tangent is refused).  ``turned``: weight is [K, N].  ``x8``: f8_rows(x) where the caller has it already.  K and N
     are 2^22 at most, and so are the rows where weight or bias wants a gradient.
     Error of an operand: half a step of e4m3, 2^-4 of a value, plus 2^-10 of its block's scale for
-    small ones.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
+    small ones.  Products add as lcf_f8_gemm does for the type that they are stored in: y and dx, of x's
+    type, in fp32 for float32 rows and on the 8-bit matrix instruction for 16-bit ones (2^-10 of the sum of
+    magnitudes at most, 1.5e-5 of the result on random data, beside a store's 2^-8 or 2^-11); dW goes by
+    the weight's type.  include/lcf.h: lcf_f8_quant, lcf_f8_gemm."""
     if x.dim() == 2:
         return _lib.row_ops().f8_linear(x, weight, bias, turned, x8)
     rows = x.flatten(0, -2) if x.dim() > 2 else x.unsqueeze(0)  # (-1 is ambiguous where K = 0)
