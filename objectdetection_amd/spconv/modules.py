@@ -48,8 +48,8 @@ class RMSNorm(nn.RMSNorm):
     training and inference and for any number of rows.  eps None: 2^-23, float32's epsilon, for rows of
     every type, which is what nn.RMSNorm computes (the sums are float32's whatever the rows' type)."""
 
-    def __init__(self, num_features, eps=None, elementwise_affine=True):
-        super().__init__(num_features, eps, elementwise_affine)
+    def __init__(self, num_features, eps=None, elementwise_affine=True, device=None, dtype=None):
+        super().__init__(num_features, eps, elementwise_affine, device, dtype)
 
     def _eps(self):
         return torch.finfo(torch.float32).eps if self.eps is None else self.eps

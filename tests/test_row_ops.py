@@ -201,3 +201,13 @@ def test_long_sums_of_few_rows_are_split_where_there_is_room():
         assert L.lcf_f8_gemm_split_bytes(M, N, K, 0) == L.lcf_f8_gemm_workspace_bytes(M, N, K, 0)
     last = (1 << 31) - 1
     assert L.lcf_f8_gemm_split_bytes(last, last, 64, 0) == 0 and L.lcf_f8_gemm_split_bytes(0, 5, 64, 0) == 0
+
+
+def test_rms_norm_module_takes_what_nn_rms_norm_takes():
+    from torch import nn
+
+    from objectdetection_amd import spconv
+    for kw in (dict(), dict(eps=1e-5), dict(elementwise_affine=False), dict(device="cpu", dtype=torch.bfloat16)):
+        a, b = spconv.RMSNorm(24, **kw), nn.RMSNorm(24, **kw)
+        assert a.eps == b.eps and list(a.state_dict()) == list(b.state_dict())
+        assert a.weight is b.weight is None or (a.weight.dtype == b.weight.dtype and torch.equal(a.weight, b.weight))
